@@ -402,6 +402,63 @@ enum {
 };
 int ppml_hip_q8_last_path(void);
 
+/* ---- around an attention block ---------------------------------------------------------------
+ * Operators that a block's projections are trained and served with; no counterpart in the reference.  Element types: */
+enum {
+    PPML_ELEM_F32 = 0,
+    PPML_ELEM_F16 = 1,
+    PPML_ELEM_BF16 = 2,
+    PPML_ELEM_I8 = 3
+};
+
+/* Rows of x (rows x K, x_stride elements apart) in 8-bit integers, one scale a row: scale = max |x| times the binary32
+ * number nearest to 1/127, q = x / scale (binary32) rounded to the nearest whole number, halves to even, 0 where the scale is 0.  A row that holds an infinity or a NaN has a scale of
+ * NaN and zeros.  q_stride = i8_weight_row_bytes_hip(K): the rows are padded with zeros, as mul_mat_i8_hip takes its weight;
+ * otherwise K values a row are written, whatever lies between rows stays.  type: F32, F16 or BF16.  K <= 131071. */
+int quantize_rows_i8_hip(const void *x, int type, int64_t x_stride, int8_t *q, int64_t q_stride, float *scale, int64_t rows, int K, ppml_hip_stream_t stream);
+/* Bytes of a row of a weight as mul_mat_i8_hip takes it: K up to a multiple of 128 (0: no such K) */
+size_t i8_weight_row_bytes_hip(int K);
+/* Rows of a weight of int8 values (M x K, w_stride bytes apart) laid out like that: M * i8_weight_row_bytes_hip(K) bytes, 16-byte aligned */
+int i8_weight_pack_hip(const int8_t *w, int64_t w_stride, int M, int K, int8_t *packed, ppml_hip_stream_t stream);
+/* y[n * M + m] = (sum_k q[n][k] w[m][k]) * x_scale[n] * w_scale[m] + (bias ? bias[m] : 0), rounded to y_type (F32, F16 or BF16).  x (N x K, x_stride elements
+ * apart) is F32, F16 or BF16 and quantized by the rule above on the way (x_scale is not read), or I8 with its x_scale.  The sums are exact.  A token
+ * whose scale is NaN is NaN throughout.  The workspace, mul_mat_i8_workspace_hip(N, K) bytes, 16-byte aligned, is the call's until its work has run. */
+size_t mul_mat_i8_workspace_hip(int N, int K);
+int mul_mat_i8_hip(const int8_t *packed, const float *w_scale, const void *x, int x_type, int64_t x_stride, const float *x_scale, const float *bias,
+                   void *y, int y_type, int M, int N, int K, void *workspace, size_t workspace_bytes, ppml_hip_stream_t stream);
+
+/* Norms of queries and keys for each head with the position rotation.  A head is d consecutive elements (d <= 512); batch b, token l, head h begins at
+ * b * strides[0] + l * strides[1] + h * strides[2], in elements.  The first `rot` elements (an even number) of every head are turned, as pairs (i, i + rot / 2),
+ * or (2 i, 2 i + 1) where `interleaved` is not 0, by the token's position times freqs[i] (rot / 2 radians a position, binary64).  Positions: int32 (position_bytes 4) or int64 (8), of batch b and
+ * token l at b * position_stride + l; position_bytes 0: l.  hq or hk may be 0 (its pointers are not looked at then).
+ *   y = turn(x / sqrt(mean(x^2) + eps) * w)        w (d values, binary32) may be NULL: ones
+ * All arithmetic is binary32, the angles' binary64; one rounding to `type` on the way out. */
+typedef struct ppml_qk_norm_desc {
+    int64_t B, L;
+    int32_t hq, hk, d, rot;
+    int32_t type, interleaved, position_bytes;
+    float eps;
+    int64_t position_stride;
+    int64_t q_strides[3], k_strides[3];           /* q and k */
+    int64_t q_out_strides[3], k_out_strides[3];   /* the normed ones, or (backward) the gradients of q and k */
+    int64_t dq_strides[3], dk_strides[3];         /* backward: the gradients that come in */
+} ppml_qk_norm_desc;
+int qk_norm_rope_hip(const ppml_qk_norm_desc *desc, const void *q, const void *k, const float *wq, const float *wk, const double *freqs, const void *positions,
+                     void *q_out, void *k_out, ppml_hip_stream_t stream);
+/* Its gradients: of q and k, and of wq and wk where wq_grad / wk_grad are not NULL (they then need the workspace, which is the call's until its work has run). */
+size_t qk_norm_rope_back_workspace_hip(const ppml_qk_norm_desc *desc);
+int qk_norm_rope_back_hip(const ppml_qk_norm_desc *desc, const void *dq, const void *dk, const void *q, const void *k, const float *wq, const float *wk, const double *freqs,
+                          const void *positions, void *q_grad, void *k_grad, float *wq_grad, float *wk_grad, void *workspace, size_t workspace_bytes,
+                          ppml_hip_stream_t stream);
+
+/* Updates orthogonalised by Newton-Schulz products: X = g / (|g| + eps), then `steps` (1 to 32) times A = X X^T, X <- a X + (b A + c A A) X, on each of
+ * `batch` dense matrices of rows x cols (both up to 2^20; a matrix with more rows than columns is worked on transposed, which gives the same).  |g| is the Frobenius norm.  g and
+ * out may be the same.  Binary32-grade arithmetic for every type; one rounding on the way out.  A matrix that holds an infinity or a NaN is NaN throughout.
+ * The workspace, newton_schulz_workspace_hip bytes, 256-byte aligned, is the call's until its work has run. */
+size_t newton_schulz_workspace_hip(int64_t batch, int64_t rows, int64_t cols);
+int newton_schulz_hip(const void *g, void *out, int type, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps,
+                      void *workspace, size_t workspace_bytes, ppml_hip_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

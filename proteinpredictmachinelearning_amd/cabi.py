@@ -50,6 +50,16 @@ SIGNATURES = {
     "bcast_elemwise_hip": (_i, [_vp, _vp, _vp, _i64, _i64, _i64, _i, _vp]),
     "softmax_hip": (_i, [_vp, _vp, _i, _i, _vp]),
     "softmax_add_hip": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
+    "quantize_rows_i8_hip": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i64, _i, _vp]),
+    "i8_weight_row_bytes_hip": (C.c_size_t, [_i]),
+    "i8_weight_pack_hip": (_i, [_vp, _i64, _i, _i, _vp, _vp]),
+    "mul_mat_i8_workspace_hip": (C.c_size_t, [_i, _i]),
+    "mul_mat_i8_hip": (_i, [_vp, _vp, _vp, _i, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp, C.c_size_t, _vp]),
+    "qk_norm_rope_hip": (_i, [_vp] * 10),
+    "qk_norm_rope_back_workspace_hip": (C.c_size_t, [_vp]),
+    "qk_norm_rope_back_hip": (_i, [_vp] * 14 + [C.c_size_t, _vp]),
+    "newton_schulz_workspace_hip": (C.c_size_t, [_i64] * 3),
+    "newton_schulz_hip": (_i, [_vp, _vp, _i] + [_i64] * 3 + [_i] + [_f] * 4 + [_vp, C.c_size_t, _vp]),
     "ppml_hip_mulmat_stats": (_i, [C.POINTER(_i64), _i]),
     "ppml_hip_mulmat_stats_enable": (_i, [_i]),
     "ppml_hip_mulmat_stats_rows": (_i, [_vp, _i]),
@@ -63,6 +73,13 @@ class MulMatStat(C.Structure):
     """``ppml_hip_mulmat_stat`` of include/ppml_hip.h."""
     _fields_ = [("path", C.c_char * 32), ("M", C.c_int64), ("K", C.c_int64), ("N", C.c_int64),
                 ("calls", C.c_int64), ("ms", C.c_double)]
+
+
+class QkNormDesc(C.Structure):
+    """``ppml_qk_norm_desc`` of include/ppml_hip.h."""
+    _fields_ = [("B", C.c_int64), ("L", C.c_int64), ("hq", C.c_int32), ("hk", C.c_int32), ("d", C.c_int32), ("rot", C.c_int32),
+                ("type", C.c_int32), ("interleaved", C.c_int32), ("position_bytes", C.c_int32), ("eps", C.c_float), ("position_stride", C.c_int64)] + \
+               [(name, C.c_int64 * 3) for name in ("q_strides", "k_strides", "q_out_strides", "k_out_strides", "dq_strides", "dk_strides")]
 
 
 # every symbol include/ppml_hip_backend.h declares (the executor driver above the launchers)

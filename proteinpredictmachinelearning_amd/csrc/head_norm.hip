@@ -1,0 +1,450 @@
+// Norms of queries and keys for each head with the position rotation (qk_norm_rope_hip, qk_norm_rope_back_hip): from the
+// projection's layout, a token's heads side by side, into attention's [B][h][L][d], and the gradients back.
+//
+// One head x of one token at position p, weights w, frequencies f (radians a position):
+//   s = 1 / sqrt(mean(x^2) + eps)    n = x s    u = n w    y = R(p) u
+// R turns the pairs (i, i + rot/2), or (2i, 2i+1) where they are interleaved, by p f_i; elements from rot on stay.
+//   backward: v = R^T dy    dw = sum of v n    g = v w    dx = s (g - n mean(g n))
+//
+// Angles: p f_i may be millions of radians, of which binary32 would keep none of the fraction.  In units of a quarter turn,
+// in 64 bits, the whole number (modulo 4) picks the quadrant and the rest, at most 1/2, becomes an angle of at most pi / 4 in binary32;
+// sine and cosine there are their series up to the 11th and 10th power (next term below 2^-27 of the result).
+//
+// A group of G lanes takes a token and walks over its heads; each lane keeps its pairs' sines, cosines and weights.
+#include "elements.hpp"
+
+namespace ppmlhip {
+namespace {
+
+struct HeadSide {             // queries or keys
+    const void* x;
+    const void* dy;           // backward
+    void* out;                // y, or dx
+    const float* w;           // or null: ones
+    int64_t x_b, x_l, x_h, dy_b, dy_l, dy_h, out_b, out_l, out_h;      // elements from batch to batch, token to token, head to head
+    int heads;
+};
+struct HeadNorm {
+    HeadSide side[2];
+    const double* freqs;
+    const void* positions;    // null: a token's place in its sequence
+    int64_t pos_b;
+    int pos_type;
+    int64_t tokens;           // B L
+    int L, d, rot, interleaved;
+    float eps;
+    int group;                // lanes per token: a power of two
+    int heads_per_part;       // heads of queries and keys in one list, cut into gridDim.y parts
+    float* partial;           // backward: [work-group][2][d]
+};
+
+// sine and cosine of p f, f in quarter turns a position
+__device__ __forceinline__ void turn_of(double p, double f, float& sine, float& cosine) {
+    const double t = p * f, whole = __builtin_rint(t);
+    const float a = static_cast<float>((t - whole) * 1.5707963267948966), z = a * a;
+    float s = -2.50521083854417188e-8f;
+    s = fmaf(s, z, 2.75573192239858907e-6f);
+    s = fmaf(s, z, -1.98412698412698413e-4f);
+    s = fmaf(s, z, 8.33333333333333333e-3f);
+    s = fmaf(s, z, -1.66666666666666667e-1f);
+    s = fmaf(s * z, a, a);
+    float c = -2.75573192239858907e-7f;
+    c = fmaf(c, z, 2.48015873015873016e-5f);
+    c = fmaf(c, z, -1.38888888888888889e-3f);
+    c = fmaf(c, z, 4.16666666666666667e-2f);
+    c = fmaf(c, z, -0.5f);
+    c = fmaf(c, z, 1.0f);
+    // (of a whole number of quarter turns the remainder modulo 4; beyond 2^53 it is a multiple of two)
+    const int quarter = static_cast<int>(whole - 4.0 * __builtin_floor(whole * 0.25));
+    const float x = quarter & 1 ? c : s, y = quarter & 1 ? s : c;
+    sine = quarter & 2 ? -x : x;
+    cosine = ((quarter + 1) & 2) ? -y : y;
+}
+
+// the sum over a group of lanes, in all of them
+__device__ __forceinline__ float group_sum(float v, int group) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#define PPML_DPP(CTRL) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true))
+    if (group > 1) PPML_DPP(0xb1);                      // quad_perm [1, 0, 3, 2]
+    if (group > 2) PPML_DPP(0x4e);                      // quad_perm [2, 3, 0, 1]
+    if (group > 4) PPML_DPP(0x141);                     // row_half_mirror
+    if (group > 8) PPML_DPP(0x140);                     // row_mirror
+#undef PPML_DPP
+    if (group > 16) v = fold16(v, v, [](float a, float b) { return a + b; });
+    if (group > 32) v = fold32(v, v, [](float a, float b) { return a + b; });
+#endif
+    return v;
+}
+
+// What a lane holds of a head: R chunks of two times V elements.  A chunk's halves `a`, `b` are V pairs' first and second
+// elements (half-split) or 2 V consecutive elements (interleaved, and behind the rotated ones).
+template <int V, int R>
+struct Chunks {
+    int at_a[R], at_b[R];     // -1: outside the head
+    float sine[R][V], cosine[R][V];
+
+    __device__ __forceinline__ void place(int lane, int group, int d, int rot, bool interleaved) {
+        const int half = rot / 2, turning = interleaved ? 0 : half / V;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int c = lane + r * group;
+            if (c < turning) {
+                at_a[r] = c * V;
+                at_b[r] = half + c * V;
+            } else {
+                at_a[r] = 2 * V * c;                    // (half-split: 2 V turning = rot)
+                at_b[r] = at_a[r] + V;
+            }
+            if (at_a[r] >= d) at_a[r] = -1;
+            if (at_b[r] >= d) at_b[r] = -1;
+        }
+    }
+    __device__ __forceinline__ void angles(int lane, int group, const HeadNorm& p, double position) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int pair = (lane + r * group) * V + v;
+                sine[r][v] = 0.0f;
+                cosine[r][v] = 1.0f;
+                if (pair < p.rot / 2) turn_of(position, p.freqs[pair] * 0.63661977236758134308, sine[r][v], cosine[r][v]);
+            }
+    }
+    template <bool INTER, bool BACK>
+    __device__ __forceinline__ void rotate(float (&a)[R][V], float (&b)[R][V]) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float sn = BACK ? -sine[r][v] : sine[r][v], cs = cosine[r][v];
+                float& x = INTER && V > 1 ? (2 * v < V ? a[r][(2 * v) % V] : b[r][(2 * v) % V]) : a[r][v];
+                float& y = INTER && V > 1 ? (2 * v + 1 < V ? a[r][(2 * v + 1) % V] : b[r][(2 * v + 1) % V]) : b[r][v];
+                const float t = x * cs - y * sn;
+                y = fmaf(y, cs, x * sn);
+                x = t;
+            }
+    }
+    template <class T>
+    __device__ __forceinline__ void load(const T* head, float (&a)[R][V], float (&b)[R][V], float fill = 0.0f) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) a[r][v] = b[r][v] = fill;
+            if (at_a[r] >= 0) load_f32<T, V>(head + at_a[r], a[r]);
+            if (at_b[r] >= 0) load_f32<T, V>(head + at_b[r], b[r]);
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ void store(T* head, const float (&a)[R][V], const float (&b)[R][V]) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (at_a[r] >= 0) store_f32<T, V>(head + at_a[r], a[r]);
+            if (at_b[r] >= 0) store_f32<T, V>(head + at_b[r], b[r]);
+        }
+    }
+};
+
+__device__ __forceinline__ double position_of(const HeadNorm& p, int64_t b, int64_t l) {
+    if (!p.positions) return static_cast<double>(l);
+    const int64_t at = b * p.pos_b + l;
+    return p.pos_type == 4 ? static_cast<double>(static_cast<const int32_t*>(p.positions)[at])
+                           : static_cast<double>(static_cast<const int64_t*>(p.positions)[at]);
+}
+
+template <class T, int V, int R, bool INTER>
+__global__ __launch_bounds__(256) void head_norm_kernel(const HeadNorm p) {
+    const int lane = threadIdx.x & (p.group - 1);
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * (256 / p.group) + threadIdx.x / p.group;
+    if (token >= p.tokens) return;                      // (whole groups)
+    const int64_t b = token / p.L, l = token % p.L;
+    Chunks<V, R> ch;
+    ch.place(lane, p.group, p.d, p.rot, INTER);
+    ch.angles(lane, p.group, p, position_of(p, b, l));
+    const int all = p.side[0].heads + p.side[1].heads;
+    const int first = blockIdx.y * p.heads_per_part, end = first + p.heads_per_part < all ? first + p.heads_per_part : all;
+    const float mean = 1.0f / static_cast<float>(p.d);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const HeadSide& side = p.side[s];
+        const int before = s == 0 ? 0 : p.side[0].heads;
+        int h = first - before > 0 ? first - before : 0;
+        const int stop = end - before < side.heads ? end - before : side.heads;
+        if (h >= stop) continue;
+        float wa[R][V], wb[R][V];
+        if (side.w) ch.load(side.w, wa, wb);
+        const T* const x = static_cast<const T*>(side.x) + b * side.x_b + l * side.x_l;
+        T* const y = static_cast<T*>(side.out) + b * side.out_b + l * side.out_l;
+        for (; h < stop; ++h) {
+            float xa[R][V], xb[R][V];
+            ch.load(x + h * side.x_h, xa, xb);
+            float squares = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int v = 0; v < V; ++v) squares = fmaf(xa[r][v], xa[r][v], fmaf(xb[r][v], xb[r][v], squares));
+            const float scale = rsqrtf(fmaf(group_sum(squares, p.group), mean, p.eps));
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    xa[r][v] *= side.w ? scale * wa[r][v] : scale;
+                    xb[r][v] *= side.w ? scale * wb[r][v] : scale;
+                }
+            ch.template rotate<INTER, false>(xa, xb);
+            ch.store(y + h * side.out_h, xa, xb);
+        }
+    }
+}
+
+template <class T, int V, int R, bool INTER>
+__global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];      // [tokens of the work-group][d]
+    const int lane = threadIdx.x & (p.group - 1), groups = 256 / p.group, mine = threadIdx.x / p.group;
+    Chunks<V, R> ch;
+    ch.place(lane, p.group, p.d, p.rot, INTER);
+    const int all = p.side[0].heads + p.side[1].heads;
+    const int first = blockIdx.y * p.heads_per_part, end = first + p.heads_per_part < all ? first + p.heads_per_part : all;
+    const float mean = 1.0f / static_cast<float>(p.d);
+    float dwa[2][R][V] = {}, dwb[2][R][V] = {};
+    for (int64_t token = static_cast<int64_t>(blockIdx.x) * groups + mine; token < p.tokens; token += static_cast<int64_t>(gridDim.x) * groups) {
+        const int64_t b = token / p.L, l = token % p.L;
+        ch.angles(lane, p.group, p, position_of(p, b, l));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const HeadSide& side = p.side[s];
+            const int before = s == 0 ? 0 : p.side[0].heads;
+            int h = first - before > 0 ? first - before : 0;
+            const int stop = end - before < side.heads ? end - before : side.heads;
+            if (h >= stop) continue;
+            float wa[R][V], wb[R][V];
+            if (side.w) ch.load(side.w, wa, wb);
+            const T* const x = static_cast<const T*>(side.x) + b * side.x_b + l * side.x_l;
+            const T* const dy = static_cast<const T*>(side.dy) + b * side.dy_b + l * side.dy_l;
+            T* const dx = static_cast<T*>(side.out) + b * side.out_b + l * side.out_l;
+            for (; h < stop; ++h) {
+                float xa[R][V], xb[R][V], ga[R][V], gb[R][V];
+                ch.load(x + h * side.x_h, xa, xb);
+                ch.load(dy + h * side.dy_h, ga, gb);
+                float squares = 0.0f;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) squares = fmaf(xa[r][v], xa[r][v], fmaf(xb[r][v], xb[r][v], squares));
+                const float scale = rsqrtf(fmaf(group_sum(squares, p.group), mean, p.eps));
+                ch.template rotate<INTER, true>(ga, gb);
+                float along = 0.0f;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        xa[r][v] *= scale;
+                        xb[r][v] *= scale;
+                        if (side.w) {
+                            dwa[s][r][v] = fmaf(ga[r][v], xa[r][v], dwa[s][r][v]);
+                            dwb[s][r][v] = fmaf(gb[r][v], xb[r][v], dwb[s][r][v]);
+                            ga[r][v] *= wa[r][v];
+                            gb[r][v] *= wb[r][v];
+                        }
+                        along = fmaf(ga[r][v], xa[r][v], fmaf(gb[r][v], xb[r][v], along));
+                    }
+                along = group_sum(along, p.group) * mean;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        ga[r][v] = scale * fmaf(-xa[r][v], along, ga[r][v]);
+                        gb[r][v] = scale * fmaf(-xb[r][v], along, gb[r][v]);
+                    }
+                ch.store(dx + h * side.out_h, ga, gb);
+            }
+        }
+    }
+    // the work-group's sums of dw, tokens in their order
+    if (!p.partial) return;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if (!p.side[s].w) continue;
+        __syncthreads();
+        ch.store(lds + mine * p.d, dwa[s], dwb[s]);
+        __syncthreads();
+        for (int e = threadIdx.x; e < p.d; e += 256) {
+            float sum = 0.0f;
+            for (int g = 0; g < groups; ++g) sum += lds[g * p.d + e];
+            p.partial[(static_cast<int64_t>(blockIdx.y * gridDim.x + blockIdx.x) * 2 + s) * p.d + e] = sum;
+        }
+    }
+}
+
+// dw[e] = the sum over `parts` work-groups of partial[part][side][e]: 16 threads per element, each a run of parts in their order
+__global__ __launch_bounds__(256) void head_norm_weights_kernel(const float* partial, int parts, int d, float* dwq, float* dwk) {
+    __shared__ float lds[16][17];
+    const int col = threadIdx.x & 15, run = threadIdx.x >> 4;
+    const int e = blockIdx.x * 16 + col, s = blockIdx.y;
+    float* const dw = s == 0 ? dwq : dwk;
+    if (!dw) return;
+    float sum = 0.0f;
+    if (e < d)
+        for (int i = run; i < parts; i += 16) sum += partial[(static_cast<int64_t>(i) * 2 + s) * d + e];
+    lds[run][col] = sum;
+    __syncthreads();
+    if (run == 0 && e < d) {
+        for (int i = 1; i < 16; ++i) sum += lds[i][col];
+        dw[e] = sum;
+    }
+}
+
+constexpr int HEAD_MAX_D = 512;
+constexpr int BACK_MOST_BLOCKS = 1024;
+
+struct HeadPlan { bool vec; int chunks, group, chunks_per_lane; unsigned blocks, parts; };
+
+size_t elem_bytes(int type) { return type == PPML_ELEM_F32 ? 4 : 2; }
+
+// how a head is dealt to lanes: the layout allows four elements at a time, or one
+HeadPlan plan_heads(const ppml_qk_norm_desc& a, bool aligned, bool back) {
+    HeadPlan pl{};
+    const bool whole = a.interleaved ? a.d % 8 == 0 && a.rot % 8 == 0 : a.rot % 8 == 0 && (a.d - a.rot) % 8 == 0;
+    pl.vec = aligned && whole;
+    pl.chunks = pl.vec ? a.d / 8 : (a.d + 1) / 2;
+    pl.group = 1;
+    while (pl.group < 64 && pl.group < pl.chunks) pl.group *= 2;
+    pl.chunks_per_lane = (pl.chunks + pl.group - 1) / pl.group;
+    const int64_t tokens = a.B * a.L, per_block = 256 / pl.group;
+    int64_t blocks = (tokens + per_block - 1) / per_block;
+    const int heads = a.hq + a.hk;
+    if (back && blocks > BACK_MOST_BLOCKS) blocks = BACK_MOST_BLOCKS;
+    int64_t parts = 1;
+    while (parts < heads && blocks * parts < 1024) ++parts;
+    pl.blocks = static_cast<unsigned>(blocks);
+    pl.parts = static_cast<unsigned>(parts);
+    return pl;
+}
+
+bool desc_ok(const ppml_qk_norm_desc* a) {
+    return a && a->B > 0 && a->L > 0 && a->B <= INT64_MAX / a->L && a->L <= 0x7fffffff && a->hq >= 0 && a->hk >= 0 && a->hq + static_cast<int64_t>(a->hk) > 0 && a->hq <= 65535 && a->hk <= 65535 &&
+           a->d > 0 && a->d <= HEAD_MAX_D && a->rot >= 0 && a->rot <= a->d && a->rot % 2 == 0 &&
+           (a->type == PPML_ELEM_F32 || a->type == PPML_ELEM_F16 || a->type == PPML_ELEM_BF16) && a->eps >= 0.0f &&
+           (a->position_bytes == 0 || a->position_bytes == 4 || a->position_bytes == 8) && a->B * a->L <= (int64_t{1} << 32);
+}
+
+bool side_aligned(const HeadSide& s, size_t elem, bool back) {
+    if (s.heads == 0) return true;
+    const uintptr_t bytes = 4 * elem;
+    const auto ok = [&](const void* ptr, int64_t b, int64_t l, int64_t h) {
+        return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && b % 4 == 0 && l % 4 == 0 && h % 4 == 0;
+    };
+    return ok(s.x, s.x_b, s.x_l, s.x_h) && ok(s.out, s.out_b, s.out_l, s.out_h) && (!back || ok(s.dy, s.dy_b, s.dy_l, s.dy_h)) &&
+           reinterpret_cast<uintptr_t>(s.w) % 16 == 0;
+}
+
+template <class T, int V, int R>
+void launch_heads(const HeadNorm& p, const HeadPlan& pl, bool back, hipStream_t stream) {
+    const dim3 grid(pl.blocks, pl.parts), block(256);
+    const size_t lds = back ? static_cast<size_t>(256 / p.group) * p.d * 4 : 0;
+    if (back) {
+        if (p.interleaved) hipLaunchKernelGGL((head_norm_back_kernel<T, V, R, true>), grid, block, lds, stream, p);
+        else               hipLaunchKernelGGL((head_norm_back_kernel<T, V, R, false>), grid, block, lds, stream, p);
+    } else {
+        if (p.interleaved) hipLaunchKernelGGL((head_norm_kernel<T, V, R, true>), grid, block, 0, stream, p);
+        else               hipLaunchKernelGGL((head_norm_kernel<T, V, R, false>), grid, block, 0, stream, p);
+    }
+}
+
+template <class T>
+void launch_heads(const HeadNorm& p, const HeadPlan& pl, bool back, hipStream_t stream) {
+    if (pl.vec) launch_heads<T, 4, 1>(p, pl, back, stream);
+    else if (pl.chunks_per_lane == 1) launch_heads<T, 1, 1>(p, pl, back, stream);
+    else launch_heads<T, 1, 4>(p, pl, back, stream);
+}
+
+int run_heads(const ppml_qk_norm_desc& a, HeadNorm p, const HeadPlan& pl, bool back, hipStream_t stream, const char* what) {
+    p.group = pl.group;
+    p.heads_per_part = (a.hq + a.hk + static_cast<int>(pl.parts) - 1) / static_cast<int>(pl.parts);
+    switch (a.type) {
+        case PPML_ELEM_F32: launch_heads<float>(p, pl, back, stream); break;
+        case PPML_ELEM_F16: launch_heads<_Float16>(p, pl, back, stream); break;
+        default:            launch_heads<__bf16>(p, pl, back, stream); break;
+    }
+    return check_launch(what);
+}
+
+HeadNorm describe(const ppml_qk_norm_desc& a, const double* freqs, const void* positions) {
+    HeadNorm p{};
+    p.freqs = freqs;
+    p.positions = a.position_bytes ? positions : nullptr;
+    p.pos_b = a.position_stride;
+    p.pos_type = a.position_bytes;
+    p.tokens = a.B * a.L;
+    p.L = static_cast<int>(a.L);
+    p.d = a.d;
+    p.rot = a.rot;
+    p.interleaved = a.interleaved;
+    p.eps = a.eps;
+    return p;
+}
+
+HeadSide side_of(const void* x, const int64_t* xs, const void* dy, const int64_t* dys, void* out, const int64_t* outs, const float* w, int heads) {
+    HeadSide s{};
+    s.x = x; s.dy = dy; s.out = out; s.w = w; s.heads = heads;
+    s.x_b = xs[0]; s.x_l = xs[1]; s.x_h = xs[2];
+    if (dys) { s.dy_b = dys[0]; s.dy_l = dys[1]; s.dy_h = dys[2]; }
+    s.out_b = outs[0]; s.out_l = outs[1]; s.out_h = outs[2];
+    return s;
+}
+
+}  // namespace
+}  // namespace ppmlhip
+
+using namespace ppmlhip;
+
+extern "C" int qk_norm_rope_hip(const ppml_qk_norm_desc* a, const void* q, const void* k, const float* wq, const float* wk, const double* freqs,
+                                const void* positions, void* q_out, void* k_out, ppml_hip_stream_t stream) {
+    if (!desc_ok(a) || (a->hq > 0 && (!q || !q_out)) || (a->hk > 0 && (!k || !k_out)) || (a->rot > 0 && !freqs) || (a->position_bytes > 0 && !positions)) {
+        set_error("qk_norm_rope_hip: bad arguments");
+        return RC_BAD_ARGS;
+    }
+    HeadNorm p = describe(*a, freqs, positions);
+    p.side[0] = side_of(q, a->q_strides, nullptr, nullptr, q_out, a->q_out_strides, wq, a->hq);
+    p.side[1] = side_of(k, a->k_strides, nullptr, nullptr, k_out, a->k_out_strides, wk, a->hk);
+    const size_t elem = elem_bytes(a->type);
+    const HeadPlan pl = plan_heads(*a, side_aligned(p.side[0], elem, false) && side_aligned(p.side[1], elem, false), false);
+    return run_heads(*a, p, pl, false, static_cast<hipStream_t>(stream), "qk_norm_rope_hip");
+}
+
+extern "C" size_t qk_norm_rope_back_workspace_hip(const ppml_qk_norm_desc* a) {
+    if (!desc_ok(a)) return 0;
+    size_t most = 0;
+    for (const bool vec : {false, true}) {
+        const HeadPlan pl = plan_heads(*a, vec, true);
+        const size_t bytes = static_cast<size_t>(pl.blocks) * pl.parts * 2 * static_cast<size_t>(a->d) * 4;
+        if (bytes > most) most = bytes;
+    }
+    return most;
+}
+
+extern "C" int qk_norm_rope_back_hip(const ppml_qk_norm_desc* a, const void* dq, const void* dk, const void* q, const void* k, const float* wq, const float* wk,
+                                     const double* freqs, const void* positions, void* q_grad, void* k_grad, float* wq_grad, float* wk_grad,
+                                     void* workspace, size_t workspace_bytes, ppml_hip_stream_t stream_) {
+    const hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (!desc_ok(a) || (a->hq > 0 && (!q || !dq || !q_grad)) || (a->hk > 0 && (!k || !dk || !k_grad)) || (a->rot > 0 && !freqs) || (a->position_bytes > 0 && !positions) ||
+        (wq_grad && !wq) || (wk_grad && !wk)) {
+        set_error("qk_norm_rope_back_hip: bad arguments");
+        return RC_BAD_ARGS;
+    }
+    const bool weights = wq_grad || wk_grad;
+    if (weights && (!workspace || workspace_bytes < qk_norm_rope_back_workspace_hip(a) || (reinterpret_cast<uintptr_t>(workspace) & 3) != 0)) {
+        set_error("qk_norm_rope_back_hip: needs %zu bytes of workspace (got %zu)", qk_norm_rope_back_workspace_hip(a), workspace_bytes);
+        return RC_BAD_ARGS;
+    }
+    HeadNorm p = describe(*a, freqs, positions);
+    p.side[0] = side_of(q, a->q_strides, dq, a->dq_strides, q_grad, a->q_out_strides, wq, a->hq);
+    p.side[1] = side_of(k, a->k_strides, dk, a->dk_strides, k_grad, a->k_out_strides, wk, a->hk);
+    p.partial = weights ? static_cast<float*>(workspace) : nullptr;
+    const size_t elem = elem_bytes(a->type);
+    const HeadPlan pl = plan_heads(*a, side_aligned(p.side[0], elem, true) && side_aligned(p.side[1], elem, true), true);
+    const int rc = run_heads(*a, p, pl, true, stream, "qk_norm_rope_back_hip");
+    if (rc != RC_OK || !weights) return rc;
+    hipLaunchKernelGGL(head_norm_weights_kernel, dim3((a->d + 15) / 16, 2), dim3(256), 0, stream, static_cast<const float*>(workspace),
+                       static_cast<int>(pl.blocks * pl.parts), a->d, wq_grad, wk_grad);
+    return check_launch("qk_norm_rope_back_hip");
+}

@@ -606,3 +606,257 @@ def mul_mat_q8(w: Q8Weight, x: torch.Tensor, c_trans: int = 1, relu: bool = Fals
                                                            c_trans, (1 if relu else 0) | (2 if act == "q8_1" else 0) | _Q8_PATH_FLAGS[path],
                                                            _ptr(xq), _ptr(sums), _stream()))
     return (out, xq, sums) if dump else out
+
+
+# ----------------------------------------------------------------------------- around an attention block
+ELEM_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _operand(t, name: str, dtypes=_FLOATS) -> torch.Tensor:
+    """A tensor on the current device (whose stream the call goes to), of one of these types."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes:
+        raise TypeError(f"{name} must be a device tensor of {' / '.join(str(d)[6:] for d in dtypes)}")
+    if t.device.index != _current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
+    return t
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    # torch's allocator: kept for its next taker on the same stream, and a captured graph's own where the stream is under capture
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _rows(t: torch.Tensor):
+    """(tensor, elements from row to row) of a matrix whose rows are dense and do not overlap"""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, max(t.stride(0), t.shape[1])
+
+
+def quantize_rows_i8(x: torch.Tensor):
+    """x [..., K] (float32, float16, bfloat16) -> (q int8 of its shape, scale float32 [...]): a scale per row, max |x| times
+    1/127 in binary32, and x / scale rounded to the nearest whole number, halves to even.  A row of zeros has scale 0; one with an infinity or a NaN
+    has scale NaN and zeros."""
+    x = _operand(x, "x")
+    K = x.shape[-1] if x.dim() else 0
+    if not 1 <= K <= 131071:
+        raise ValueError(f"quantize_rows_i8: rows of 1 to 131071 elements, got {tuple(x.shape)}")
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    lib = _lib()
+    if x.numel():
+        rows, stride = _rows(x.reshape(-1, K))
+        cabi.check("quantize_rows_i8_hip", lib.quantize_rows_i8_hip(_ptr(rows), ELEM_TYPES[x.dtype], stride, _ptr(q), K, _ptr(scale), rows.shape[0], K, _stream()))
+    return q, scale
+
+
+class I8Weight:
+    """A weight [M, K] (rows = out features) in 8-bit integers, one scale a row (float32 [M]).
+
+    ``pack()`` returns the copy whose rows are padded for the product, made once per weight (a weight with K a multiple of 128 is
+    its own); ``mul_mat_i8`` packs any other per call."""
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor):
+        data, scale = _operand(data, "data", (torch.int8,)), _operand(scale, "scale", (torch.float32,))
+        if data.dim() != 2 or not 1 <= data.shape[1] <= 131071 or data.shape[0] < 1 or tuple(scale.shape) != (data.shape[0],):
+            raise ValueError(f"I8Weight: data must be [M, K] with K of 1 to 131071 and scale [M], got {tuple(data.shape)} and {tuple(scale.shape)}")
+        self.data, self.scale = data, scale.contiguous()
+        self.M, self.K = data.shape
+        self._packed = data if data.is_contiguous() and self.K % 128 == 0 and data.data_ptr() % 16 == 0 else None
+
+    @classmethod
+    def from_f32(cls, w: torch.Tensor) -> "I8Weight":
+        """Quantizes a weight of any of the float types, a scale per row."""
+        if not isinstance(w, torch.Tensor) or w.dim() != 2:
+            raise ValueError("I8Weight.from_f32: a weight is a matrix")
+        return cls(*quantize_rows_i8(w))
+
+    def pack(self) -> "I8Weight":
+        if self._packed is not None:
+            return self
+        lib = _lib()
+        data, stride = _rows(self.data)
+        out = torch.empty((self.M, lib.i8_weight_row_bytes_hip(self.K)), dtype=torch.int8, device=data.device)
+        cabi.check("i8_weight_pack_hip", lib.i8_weight_pack_hip(_ptr(data), stride, self.M, self.K, _ptr(out), _stream()))
+        packed = I8Weight(self.data, self.scale)
+        packed._packed = out
+        return packed
+
+
+def mul_mat_i8(w: I8Weight, x, bias: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Linear in 8-bit integers: x [N, K] times w [M, K] -> [N, M] (+ bias float32 [M]), one scale a token and one a channel.  x is
+    float32, float16 or bfloat16 and quantized on the way, or what quantize_rows_i8 returned (q, scale) for it, so that several layers
+    share one quantization.  The sums are exact.  dtype: of the result, x's by default (float32 for quantized x)."""
+    if not isinstance(w, I8Weight):
+        raise TypeError("mul_mat_i8: w must be an I8Weight")
+    scale = None
+    if isinstance(x, (tuple, list)):
+        if len(x) != 2:
+            raise ValueError("mul_mat_i8: quantized activations are (q, scale)")
+        x, scale = _operand(x[0], "q", (torch.int8,)), _operand(x[1], "scale", (torch.float32,))
+        if x.dim() != 2 or tuple(scale.shape) != (x.shape[0],):
+            raise ValueError(f"mul_mat_i8: q must be [N, K] and scale [N], got {tuple(x.shape)} and {tuple(scale.shape)}")
+        scale = scale.contiguous()
+    else:
+        x = _operand(x, "x")
+    if x.dim() != 2 or x.shape[1] != w.K:
+        raise ValueError(f"mul_mat_i8: activations {tuple(x.shape)} do not match weight K={w.K}")
+    dtype = dtype or (x.dtype if scale is None else torch.float32)
+    if dtype not in _FLOATS:
+        raise TypeError(f"mul_mat_i8: the result is float32, float16 or bfloat16, not {dtype}")
+    if w.data.device != x.device:
+        raise ValueError(f"mul_mat_i8: the weight is on {w.data.device}, the activations on {x.device}")
+    if bias is not None:
+        bias = _operand(bias, "bias", (torch.float32,)).contiguous()
+        if tuple(bias.shape) != (w.M,):
+            raise ValueError(f"mul_mat_i8: bias {tuple(bias.shape)}, expected ({w.M},)")
+    N, K = x.shape
+    out = torch.empty((N, w.M), dtype=dtype, device=x.device)
+    lib = _lib()
+    if N == 0:
+        return out
+    packed = w.pack()._packed
+    x, stride = _rows(x)
+    nbytes = lib.mul_mat_i8_workspace_hip(N, K)
+    ws = _workspace(nbytes, x.device)
+    cabi.check("mul_mat_i8_hip", lib.mul_mat_i8_hip(_ptr(packed), _ptr(w.scale), _ptr(x), ELEM_TYPES[x.dtype], stride, _ptr(scale), _ptr(bias), _ptr(out),
+                                                    ELEM_TYPES[dtype], w.M, N, K, _ptr(ws), nbytes, _stream()))
+    return out
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """The usual frequencies of a rotation over `rot` elements, base ** (-2 i / rot) radians a position: float64 [rot / 2]."""
+    if rot < 2 or rot % 2:
+        raise ValueError("rope_frequencies: rot must be an even number of elements, 2 or more")
+    i = torch.arange(rot // 2, dtype=torch.float64, device="cuda" if device is None else device)
+    return float(base) ** (-2.0 * i / rot)
+
+
+def _heads(t, name: str, like=None) -> torch.Tensor:
+    t = _operand(t, name, _FLOATS if like is None else (like.dtype,))
+    if t.dim() != 4:
+        raise ValueError(f"{name} must have four dimensions, got {tuple(t.shape)}")
+    return t if t.shape[3] <= 1 or t.stride(3) == 1 else t.contiguous()
+
+
+def _steps(t: torch.Tensor, dims):
+    """Elements from batch to batch, token to token, head to head (a dimension of one element is never stepped over)"""
+    return (C.c_int64 * 3)(*(t.stride(i) if t.shape[i] > 1 else 0 for i in dims))
+
+
+def _qk_norm_desc(who, q, k, wq, wk, freqs, positions, eps, interleaved):
+    q = _heads(q, "q")
+    k = _heads(k, "k", q)
+    B, L, hq, d = q.shape
+    if k.shape[0] != B or k.shape[1] != L or k.shape[3] != d:
+        raise ValueError(f"{who}: q (B, L, hq, d) {tuple(q.shape)} and k (B, L, hk, d) {tuple(k.shape)} differ in B, L or d")
+    if not 1 <= d <= 512:
+        raise ValueError(f"{who}: heads of 1 to 512 elements, got {d}")
+    if hq < 1 or k.shape[2] < 1:
+        raise ValueError(f"{who}: q and k need a head each")
+    if not eps >= 0.0:
+        raise ValueError(f"{who}: eps must not be negative")
+    weights = []
+    for w, name in ((wq, "wq"), (wk, "wk")):
+        if w is not None:
+            w = _operand(w, name, (torch.float32,)).contiguous()
+            if tuple(w.shape) != (d,):
+                raise ValueError(f"{who}: {name} {tuple(w.shape)}, expected ({d},)")
+        weights.append(w)
+    a = cabi.QkNormDesc(B=B, L=L, hq=hq, hk=k.shape[2], d=d, type=ELEM_TYPES[q.dtype], interleaved=int(bool(interleaved)), eps=eps)
+    if freqs is not None:
+        freqs = _operand(freqs, "freqs", (torch.float64,)).contiguous()
+        if freqs.dim() != 1 or 2 * freqs.shape[0] > d:
+            raise ValueError(f"{who}: freqs must be a vector of at most d / 2 = {d // 2} frequencies, got {tuple(freqs.shape)}")
+        a.rot = 2 * freqs.shape[0]
+    if positions is not None:
+        positions = _operand(positions, "positions", (torch.int32, torch.int64))
+        if tuple(positions.shape) not in ((L,), (B, L)):
+            raise ValueError(f"{who}: positions must be (L,) or (B, L), got {tuple(positions.shape)}")
+        positions = positions.contiguous()
+        a.position_bytes = positions.element_size()
+        a.position_stride = L if positions.dim() == 2 else 0
+    a.q_strides, a.k_strides = _steps(q, (0, 1, 2)), _steps(k, (0, 1, 2))
+    return a, q, k, weights[0], weights[1], freqs, positions
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None = None, wk: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+                 positions: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False):
+    """Norms of queries and keys for each head, times their weights, with the position rotation, in one pass into attention's layout:
+    q (B, L, hq, d), k (B, L, hk, d) -- slices of a fused projection's output as they are -- -> (B, hq, L, d), (B, hk, L, d).
+
+    float32, float16 or bfloat16; wq, wk float32 (d,) or None (ones).  freqs: float64 radians a position, one per pair (rope_frequencies; scaled
+    ones as a long context wants them); the first 2 * len(freqs) elements of a head are turned, as pairs (i, i + len(freqs)), or of neighbours
+    where `interleaved`; None turns nothing.  positions: int32 / int64 (B, L) or (L,); None: 0, 1, ..."""
+    a, q, k, wq, wk, freqs, positions = _qk_norm_desc("qk_norm_rope", q, k, wq, wk, freqs, positions, eps, interleaved)
+    yq, yk = (torch.empty((a.B, t.shape[2], a.L, a.d), dtype=q.dtype, device=q.device) for t in (q, k))
+    a.q_out_strides, a.k_out_strides = _steps(yq, (0, 2, 1)), _steps(yk, (0, 2, 1))
+    lib = _lib()
+    if a.B * a.L:
+        cabi.check("qk_norm_rope_hip", lib.qk_norm_rope_hip(C.byref(a), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(freqs), _ptr(positions), _ptr(yq), _ptr(yk), _stream()))
+    return yq, yk
+
+
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None = None, wk: torch.Tensor | None = None,
+                          freqs: torch.Tensor | None = None, positions: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                          out: torch.Tensor | None = None):
+    """Gradients of qk_norm_rope for dq (B, hq, L, d), dk (B, hk, L, d) and its inputs: (dq (B, L, hq, d), dk (B, L, hk, d), dwq, dwk), the last two
+    None without weights.  out: the fused projection's gradient, contiguous (B, L, C) with C >= (hq + hk) d: q's heads are then written
+    to its first columns, k's behind them, the rest (the values') stays as it is, and the first two results are views of it."""
+    a, q, k, wq, wk, freqs, positions = _qk_norm_desc("qk_norm_rope_backward", q, k, wq, wk, freqs, positions, eps, interleaved)
+    dq, dk = _heads(dq, "dq", q), _heads(dk, "dk", q)
+    for t, h, name in ((dq, a.hq, "dq"), (dk, a.hk, "dk")):
+        if tuple(t.shape) != (a.B, h, a.L, a.d):
+            raise ValueError(f"qk_norm_rope_backward: {name} {tuple(t.shape)}, expected {(a.B, h, a.L, a.d)}")
+    if out is None:
+        gq, gk = (torch.empty((a.B, a.L, h, a.d), dtype=q.dtype, device=q.device) for h in (a.hq, a.hk))
+    else:
+        out = _operand(out, "out", (q.dtype,))
+        if out.dim() != 3 or out.shape[0] != a.B or out.shape[1] != a.L or out.shape[2] < (a.hq + a.hk) * a.d or not out.is_contiguous():
+            raise ValueError(f"qk_norm_rope_backward: out must be contiguous (B, L, C) with C >= {(a.hq + a.hk) * a.d}, got {tuple(out.shape)}")
+        if out.untyped_storage().data_ptr() in [t.untyped_storage().data_ptr() for t in (q, k, dq, dk)] and out.numel():
+            raise ValueError("qk_norm_rope_backward: out must not share memory with what is read")
+        gq = out[:, :, :a.hq * a.d].unflatten(2, (a.hq, a.d))
+        gk = out[:, :, a.hq * a.d:(a.hq + a.hk) * a.d].unflatten(2, (a.hk, a.d))
+    a.q_out_strides, a.k_out_strides = _steps(gq, (0, 1, 2)), _steps(gk, (0, 1, 2))
+    a.dq_strides, a.dk_strides = _steps(dq, (0, 2, 1)), _steps(dk, (0, 2, 1))
+    lib = _lib()
+    if not a.B * a.L:
+        return gq, gk, None if wq is None else torch.zeros_like(wq), None if wk is None else torch.zeros_like(wk)
+    dwq, dwk = (None if w is None else torch.empty_like(w) for w in (wq, wk))
+    nbytes = lib.qk_norm_rope_back_workspace_hip(C.byref(a)) if wq is not None or wk is not None else 0
+    ws = _workspace(nbytes, q.device) if nbytes else None
+    cabi.check("qk_norm_rope_back_hip",
+               lib.qk_norm_rope_back_hip(C.byref(a), _ptr(dq), _ptr(dk), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(freqs), _ptr(positions), _ptr(gq), _ptr(gk),
+                                         _ptr(dwq), _ptr(dwk), _ptr(ws), nbytes, _stream()))
+    return gq, gk, dwq, dwk
+
+
+NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
+    """An update orthogonalised by Newton-Schulz products: X = g / (|g| + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T,
+    for every matrix of g [..., rows, cols] (float32, float16, bfloat16; binary32-grade arithmetic for all) -> the same shape and type.
+    Singular values above a hundredth or so of the largest come out near 1.  coefficients: (a, b, c)."""
+    g = _operand(g, "g")
+    if g.dim() < 2:
+        raise ValueError(f"newton_schulz: g must be a matrix or a stack of them, got {tuple(g.shape)}")
+    a, b, c = (float(x) for x in coefficients)
+    if not 1 <= int(steps) <= 32 or not all(map(math.isfinite, (a, b, c, eps))) or eps < 0:
+        raise ValueError("newton_schulz: 1 to 32 steps, finite coefficients, eps finite and not negative")
+    g = g.contiguous()
+    out = torch.empty_like(g)
+    lib = _lib()
+    if g.numel() == 0:
+        return out
+    rows, cols = g.shape[-2:]
+    batch = g.numel() // (rows * cols)
+    nbytes = lib.newton_schulz_workspace_hip(batch, rows, cols)
+    if nbytes == 0:
+        raise ValueError(f"newton_schulz: at most 65535 matrices with sides up to 2^20, got {tuple(g.shape)}")
+    ws = _workspace(nbytes, g.device)
+    cabi.check("newton_schulz_hip", lib.newton_schulz_hip(_ptr(g), _ptr(out), ELEM_TYPES[g.dtype], batch, rows, cols, int(steps), a, b, c, float(eps), _ptr(ws), nbytes,
+                                                          _stream()))
+    return out

@@ -1,0 +1,122 @@
+"""The operators around an attention block together, as a program uses them: projection, head norms with rotation, attention,
+the way back to the projection's weight, its orthogonalised update, and the updated weight served in 8-bit integers.
+
+Against the same block in 64 bits.  Attention's bar is 1e-4 of the largest value (as its own tests have it); the projections, norms and
+their gradients add to that in proportion, so every result here is held to a few 1e-4 of its largest value."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+B, L, H, D = 4, 51, 8, 32
+WIDTH = H * D
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a device"
+    from proteinpredictmachinelearning_amd import ops as _ops
+
+    return _ops
+
+
+def heads(t):
+    return [part.unflatten(-1, (H, D)) for part in t.unflatten(0, (B, L)).chunk(3, dim=-1)]
+
+
+def near(got, want, share):
+    err = (got.double().cpu() - want).abs().max().item()
+    assert err <= share * want.abs().max().item(), f"{err / want.abs().max().item():.3e}"
+
+
+def reference(x, w, wq, wk, freqs, dy):
+    """(output, gradient of w, of wq, of wk) in 64 bits by torch's own differentiation"""
+    x, w, wq, wk, freqs, dy = (t.double().cpu() for t in (x, w, wq, wk, freqs, dy))
+    for t in (w, wq, wk):
+        t.requires_grad_()
+    q, k, v = heads(x @ w.t())
+    angle = (torch.arange(L).double()[:, None] * freqs)[:, None]
+
+    def turn(u):
+        a, b = u.chunk(2, dim=-1)
+        return torch.cat((a * torch.cos(angle) - b * torch.sin(angle), b * torch.cos(angle) + a * torch.sin(angle)), -1)
+
+    q, k = (turn(t / torch.sqrt((t * t).mean(-1, keepdim=True) + 1e-6) * n).transpose(1, 2) for t, n in ((q, wq), (k, wk)))
+    o = torch.softmax(q @ k.transpose(-2, -1).contiguous() / math.sqrt(D), -1) @ v.transpose(1, 2).contiguous()
+    o.backward(dy)
+    return o.detach(), w.grad, wq.grad, wk.grad
+
+
+def test_a_step_of_training_and_its_weight_in_service(ops):
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(B * L, WIDTH, device="cuda", generator=gen)
+    w = torch.randn(3 * WIDTH, WIDTH, device="cuda", generator=gen) / math.sqrt(WIDTH)
+    wq, wk = (1 + 0.1 * torch.randn(D, device="cuda", generator=gen) for _ in range(2))
+    dy = torch.randn(B, H, L, D, device="cuda", generator=gen)
+    freqs = ops.rope_frequencies(D)
+    want_o, want_w, want_wq, want_wk = reference(x, w, wq, wk, freqs, dy)
+
+    def forward(project):
+        qkv = project()
+        q, k, v = heads(qkv)
+        yq, yk = ops.qk_norm_rope(q, k, wq, wk, freqs)
+        yv = v.transpose(1, 2).contiguous()
+        o, lse = ops.flash_attn_forward(yq, yk, yv)
+        return q, k, yq, yk, yv, o, lse
+
+    q, k, yq, yk, yv, o, lse = forward(lambda: ops.mul_mat(x, w))
+    near(o, want_o, 3e-4)
+    dq, dk, dv, _ = ops.flash_attn_backward(yq, yk, yv, None, o, dy, lse, want=("dq", "dk", "dv"))
+    grad = torch.empty(B, L, 3 * WIDTH, device="cuda")
+    grad[..., 2 * WIDTH:] = dv.transpose(1, 2).flatten(2)
+    _, _, gwq, gwk = ops.qk_norm_rope_backward(dq, dk, q, k, wq, wk, freqs, out=grad)
+    dw = ops.mul_mat_tn(grad.view(B * L, 3 * WIDTH), x)
+    near(dw, want_w, 5e-4)
+    near(gwq, want_wq, 5e-4)
+    near(gwk, want_wk, 5e-4)
+
+    step = ops.newton_schulz(dw)
+    # orthogonal up to what five steps give: X^T X has its eigenvalues around 1
+    values = torch.linalg.svdvals(step.double().cpu())
+    assert values.max() < 1.3 and values.median() > 0.5
+    w2 = w - 0.02 * step
+
+    served = ops.I8Weight.from_f32(w2).pack()
+    xq = ops.quantize_rows_i8(x)
+    assert torch.equal(ops.mul_mat_i8(served, xq), ops.mul_mat_i8(served, x))
+    o8 = forward(lambda: ops.mul_mat_i8(served, xq))[5]
+    o32 = forward(lambda: ops.mul_mat(x, w2))[5]
+    # a value is off by at most half a step of its row's scale: 1/254 of the largest of either operand
+    q8, s8 = (t.double().cpu() for t in xq)
+    assert ((q8 * s8[:, None] - x.double().cpu()).abs() <= 0.5001 * s8[:, None]).all()
+    near(o8, o32.double().cpu(), 0.05)
+
+
+def test_a_step_of_training_captured(ops):
+    """The whole step replayed from a graph on new activations, against the eager one"""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(B * L, WIDTH, device="cuda", generator=gen)
+    w = torch.randn(3 * WIDTH, WIDTH, device="cuda", generator=gen) / math.sqrt(WIDTH)
+    norm = torch.ones(D, device="cuda")
+    freqs = ops.rope_frequencies(D)
+    served = ops.I8Weight.from_f32(w).pack()
+
+    def step():
+        q, k, v = heads(ops.mul_mat_i8(served, x))
+        yq, yk = ops.qk_norm_rope(q, k, norm, norm, freqs)
+        gq, gk, gwq, gwk = ops.qk_norm_rope_backward(yk, yq, q, k, norm, norm, freqs)
+        return yq, yk, gq, gk, gwq, gwk, ops.newton_schulz(gq.reshape(B * L, WIDTH))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        x.normal_(generator=gen)
+        graph.replay()
+        kept = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(kept, step()))

@@ -1,0 +1,223 @@
+"""Products in 8-bit integers with one scale a token and one a channel (quantize_rows_i8, mul_mat_i8) against the definition.
+
+Quantized values and scales are equal to the rule's.  Outputs: the sum is exact, its conversion to binary32 and the
+two scales are a rounding of at most 2^-24 each, the bias another, the result's type eps / 2."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a device"
+    from proteinpredictmachinelearning_amd import ops as _ops
+
+    return _ops
+
+
+def rule(x):
+    """(q, scale) of float rows on the CPU, binary32 throughout"""
+    x = x.float().cpu().numpy()
+    largest = np.abs(x).max(axis=-1)
+    with np.errstate(all="ignore"):
+        scale = np.where(np.isfinite(largest), largest * np.float32(1 / 127), np.float32("nan")).astype(np.float32)
+        q = np.rint((x / scale[..., None]).astype(np.float32))
+    q = np.where(scale[..., None] > 0, np.clip(q, -127, 127), 0)
+    return torch.from_numpy(np.nan_to_num(q).astype(np.int8)), torch.from_numpy(scale)
+
+
+def want_and_bound(q, scale, w, w_scale, bias, dtype):
+    v = (q.double().cpu() @ w.double().cpu().t()) * scale.double().cpu()[:, None] * w_scale.double().cpu()
+    bound = 3 * 2.0 ** -24 * v.abs()
+    if bias is not None:
+        v = v + bias.double().cpu()
+        bound = bound + 2.0 ** -24 * v.abs()
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * half
+    return v, 1.01 * (bound * (1 + half) + half * v.abs()) + tiny
+
+
+def check(got, q, scale, w, w_scale, bias):
+    want, bound = want_and_bound(q, scale, w, w_scale, bias, got.dtype)
+    err = (got.double().cpu() - want).abs()
+    assert (err <= bound).all(), f"largest excess {(err - bound).max().item():.3e} of {want.abs().max().item():.3e}"
+
+
+def weight(gen, m, k):
+    return (torch.randint(-127, 128, (m, k), device="cuda", generator=gen).to(torch.int8),
+            torch.rand(m, device="cuda", generator=gen) * 0.01 + 1e-4)
+
+
+# one token to several tiles; k below, at and above a stage of 128 bytes; channels below a tile and ragged
+SHAPES = [(1, 1, 1), (1, 32, 1), (2, 127, 3), (3, 128, 130), (1, 4096, 4096), (1, 500, 1001), (7, 129, 64), (8, 1024, 257), (15, 256, 768), (16, 250, 96),
+          (17, 384, 33), (33, 96, 256), (65, 640, 200), (130, 257, 129), (408, 256, 256), (300, 1100, 300), (513, 2048, 513), (1030, 72, 24)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", SHAPES)
+def test_linear_matches_the_definition(ops, n, k, m, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(n + 7 * k + 13 * m)
+    x = (torch.randn(n, k, device="cuda", generator=gen) * torch.exp(torch.randn(n, 1, device="cuda", generator=gen))).to(dtype)
+    w, ws = weight(gen, m, k)
+    bias = torch.randn(m, device="cuda", generator=gen) if (n + k + m) % 2 else None
+    q, scale = ops.quantize_rows_i8(x)
+    want_q, want_scale = rule(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(scale.cpu(), want_scale)
+    W = ops.I8Weight(w, ws)
+    got = ops.mul_mat_i8(W.pack(), x, bias)
+    assert got.dtype == dtype and tuple(got.shape) == (n, m)
+    check(got, want_q, want_scale, w, ws, bias)
+    # the same bits from a weight that is laid out in the call, and from activations quantized ahead
+    assert torch.equal(ops.mul_mat_i8(W, x, bias), got)
+    assert torch.equal(ops.mul_mat_i8(W.pack(), (q, scale), bias, dtype=dtype), got)
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("given", TYPES)
+def test_result_type_is_free(ops, given, out):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(40, 96, device="cuda", generator=gen).to(given)
+    w, ws = weight(gen, 70, 96)
+    got = ops.mul_mat_i8(ops.I8Weight(w, ws), x, dtype=out)
+    assert got.dtype == out
+    check(got, *rule(x), w, ws, None)
+
+
+@pytest.mark.parametrize("n,k,m", [(5, 200, 64), (200, 200, 100), (40, 2100, 40)])
+def test_strided_rows(ops, n, k, m):
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    w, ws = weight(gen, m, k + 3)
+    W = ops.I8Weight(w[:, 3:], ws)                                    # a slice, its rows at odd addresses
+    big = torch.randn(n, 2 * k + 1, device="cuda", generator=gen)
+    for x in (big[:, 1:k + 1], big[:, ::2][:, :k], big[:1, :k].expand(n, k), big[:, :k].t().contiguous().t()):
+        got = ops.mul_mat_i8(W, x)
+        check(got, *rule(x), w[:, 3:], ws, None)
+        assert torch.equal(got, ops.mul_mat_i8(W.pack(), x.contiguous()))
+    q, s = ops.quantize_rows_i8(big)
+    check(ops.mul_mat_i8(W, (q[:, 5:k + 5], s)), q[:, 5:k + 5], s, w[:, 3:], ws, None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ties_zeros_and_small_rows(ops, dtype):
+    x = torch.zeros(6, 40, device="cuda")
+    x[0, :8] = torch.tensor([127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 126.5, -126.5])      # (127 r rounds to 1) ties go to the even number
+    x[2, 3] = 1e-3
+    x[3, :2] = torch.tensor([6e-8, -3e-8])                                          # subnormal halves
+    x[4] = -2.0
+    x = x.to(dtype)
+    q, scale = ops.quantize_rows_i8(x)
+    want_q, want_scale = rule(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(scale.cpu(), want_scale)
+    assert q[0, :6].tolist() == [127, 0, 2, 2, 0, -2] and scale[1] == 0
+    got = ops.mul_mat_i8(ops.I8Weight(torch.ones(3, 40, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda")), x, torch.full((3,), 0.25, device="cuda"))
+    assert (got[1] == 0.25).all()
+
+
+def test_scales_that_vanish_in_binary32(ops):
+    x = torch.zeros(3, 33, device="cuda")
+    x[0, 0], x[1, :3] = 1e-44, torch.tensor([1e-40, -1e-40, 3e-41])
+    x[2, 5] = 3.4e38
+    q, scale = ops.quantize_rows_i8(x)
+    want_q, want_scale = rule(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(scale.cpu(), want_scale)
+
+
+@pytest.mark.parametrize("n,k,m", [(4, 64, 32), (40, 300, 200), (200, 256, 256)])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_token_that_is_not_finite_is_nan_and_no_other(ops, n, k, m, bad):
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(n, k, device="cuda", generator=gen)
+    w, ws = weight(gen, m, k)
+    W = ops.I8Weight(w, ws).pack()
+    clean = ops.mul_mat_i8(W, x)
+    x[2, k - 1] = bad
+    got = ops.mul_mat_i8(W, x)
+    assert got[2].isnan().all()
+    keep = torch.arange(n, device="cuda") != 2
+    assert torch.equal(got[keep], clean[keep])
+    q, scale = ops.quantize_rows_i8(x)
+    assert scale[2].isnan() and not q[2].any()
+
+
+def test_the_largest_sums(ops):
+    k = 131071
+    x = torch.ones(2, k, device="cuda")
+    x[1] = -1.0
+    w = torch.full((3, k), 127, dtype=torch.int8, device="cuda")
+    w[1] = -128
+    got = ops.mul_mat_i8(ops.I8Weight(w, torch.ones(3, device="cuda")), x)
+    check(got, *rule(x), w, torch.ones(3), None)
+
+
+def test_rows_of_tensors_of_any_rank(ops):
+    x = torch.randn(3, 4, 5, device="cuda")
+    q, s = ops.quantize_rows_i8(x)
+    assert q.shape == x.shape and s.shape == (3, 4)
+    want_q, want_s = rule(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+    q, s = ops.quantize_rows_i8(x[0, 0])
+    assert q.shape == (5,) and s.shape == ()
+    q, s = ops.quantize_rows_i8(x[:0])
+    assert q.shape == (0, 4, 5) and s.shape == (0, 4)
+
+
+def test_no_tokens(ops):
+    W = ops.I8Weight.from_f32(torch.randn(8, 40, device="cuda"))
+    assert ops.mul_mat_i8(W, torch.empty(0, 40, device="cuda")).shape == (0, 8)
+
+
+@pytest.mark.parametrize("n", [1, 40, 600])
+def test_captured_and_replayed(ops, n):
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(n, 260, device="cuda", generator=gen)
+    W = ops.I8Weight.from_f32(torch.randn(150, 260, device="cuda", generator=gen)).pack()
+    ops.mul_mat_i8(W, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.mul_mat_i8(W, x)
+    for _ in range(4):
+        x.normal_(generator=gen)
+        graph.replay()
+        got = y.clone()
+        assert torch.equal(got, ops.mul_mat_i8(W, x))
+
+
+def test_two_streams_at_once(ops):
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    W = ops.I8Weight.from_f32(torch.randn(300, 700, device="cuda", generator=gen)).pack()
+    xs = [torch.randn(200, 700, device="cuda", generator=gen) for _ in range(2)]
+    want = [ops.mul_mat_i8(W, x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.mul_mat_i8(W, xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_refusals(ops):
+    w, ws = torch.zeros(4, 32, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    W = ops.I8Weight(w, ws)
+    x = torch.zeros(2, 32, device="cuda")
+    for bad in (lambda: ops.I8Weight(w, ws[:3]), lambda: ops.I8Weight(w[0], ws), lambda: ops.I8Weight(w[:, :0], ws),
+                lambda: ops.I8Weight.from_f32(x[0]), lambda: ops.mul_mat_i8(W, x[:, :31]), lambda: ops.mul_mat_i8(W, x[0]),
+                lambda: ops.mul_mat_i8(W, x, torch.zeros(3, device="cuda")), lambda: ops.mul_mat_i8(W, (w, ws, ws)),
+                lambda: ops.mul_mat_i8(W, (w, ws[:3])), lambda: ops.quantize_rows_i8(torch.zeros(2, 0, device="cuda")),
+                lambda: ops.quantize_rows_i8(torch.zeros(1, 131072, device="cuda"))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: ops.I8Weight(w.float(), ws), lambda: ops.I8Weight(w, ws.half()), lambda: ops.I8Weight(w.cpu(), ws), lambda: ops.mul_mat_i8(w, x),
+                lambda: ops.mul_mat_i8(W, x.double()), lambda: ops.mul_mat_i8(W, x.cpu()), lambda: ops.mul_mat_i8(W, x, dtype=torch.int8),
+                lambda: ops.mul_mat_i8(W, x, torch.zeros(4, device="cuda").half()), lambda: ops.mul_mat_i8(W, w), lambda: ops.quantize_rows_i8(w)):
+        with pytest.raises(TypeError):
+            bad()

@@ -1,0 +1,185 @@
+"""Orthogonalised updates (newton_schulz) against the iteration in 64 bits.
+
+Bound: an operand's two halves keep 2^-23 of it (rounding into them, twice), a product leaves out 2^-22 and adds in
+binary32: a walk of K roundings of 2^-24, sqrt(K) 2^-24 of the operands' size together.  Three products a step, each relative to
+the spectral norm; a step multiplies what went before by at most max |p'| = a = 3.45.  So, of the norm of the result, steps * 3 *
+a^(steps - 1) * (2^-21 + sqrt(K) 2^-24), measured in the Frobenius norm; then eps / 2 of the result's type."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+MUON = (3.4445, -4.7750, 2.0315)
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "GPU tests need a device"
+    from proteinpredictmachinelearning_amd import ops as _ops
+
+    return _ops
+
+
+def iterate(g, steps, k, eps):
+    x = g.double().cpu()
+    x = x / (torch.sqrt((x * x).sum((-2, -1), keepdim=True)) + eps)
+    a, b, c = k
+    for _ in range(steps):
+        s = x @ x.transpose(-2, -1)
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x
+
+
+def check(got, g, steps, k=MUON, eps=1e-7):
+    want = iterate(g, steps, k, eps)
+    assert got.shape == g.shape and got.dtype == g.dtype and got.is_contiguous()
+    rows, cols = g.shape[-2:]
+    half = torch.finfo(g.dtype).eps / 2
+    unit = 2.0 ** -21 + math.sqrt(max(rows, cols)) * 2.0 ** -24
+    rel = 3 * steps * max(1.0, abs(k[0])) ** (steps - 1) * unit
+    for x, y in zip(got.double().cpu().reshape(-1, rows, cols), want.reshape(-1, rows, cols)):
+        size = max(y.norm().item(), torch.linalg.matrix_norm(y, 2).item() * math.sqrt(min(rows, cols)))
+        err = (x - y).norm().item()
+        assert err <= rel * size + half * y.norm().item(), f"{err / size:.3e} against {rel:.3e}"
+
+
+def update(shape, dtype=torch.float32, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    g = torch.randn(*shape, device="cuda", generator=gen)
+    g += 3 * torch.randn(*shape[:-1], 1, device="cuda", generator=gen) * torch.randn(*shape[:-2], 1, shape[-1], device="cuda", generator=gen)
+    return (g * 1e-2).to(dtype)
+
+
+# sides of one, below and above a group of 32, a tile of 64 and of 128, either way round, stacks
+SHAPES = [(1, 1), (1, 40), (40, 1), (2, 3), (31, 33), (32, 32), (33, 64), (64, 64), (65, 31), (96, 160), (127, 129), (128, 128), (128, 512), (512, 128),
+          (130, 70), (200, 200), (256, 768), (257, 300), (384, 256), (3, 5, 7), (5, 64, 96), (2, 3, 48, 40), (4, 140, 128), (700, 260), (520, 520)]
+
+
+@pytest.mark.parametrize("steps", [1, 2, 5])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_matches_the_iteration(ops, shape, steps):
+    g = update(shape, seed=sum(shape))
+    check(ops.newton_schulz(g, steps=steps), g, steps)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(24, 72), (3, 100, 64), (160, 160)])
+def test_types(ops, shape, dtype):
+    g = update(shape, dtype, seed=1)
+    check(ops.newton_schulz(g), g, 5)
+
+
+@pytest.mark.parametrize("k", [(1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (8.2, -23.6, 17.3), (2.0, 0.0, 0.0), (0.5, 0.1, 0.0), (0.0, 1.0, -1.0), (-1.0, 0.5, 0.25)])
+@pytest.mark.parametrize("shape", [(40, 50), (150, 140)])
+def test_other_coefficients(ops, shape, k):
+    # (one step: no power of a coefficient comes in)
+    g = update(shape, seed=2)
+    check(ops.newton_schulz(g, steps=1, coefficients=k), g, 1, k)
+
+
+def test_singular_values_come_near_one(ops):
+    u, _ = torch.linalg.qr(torch.randn(160, 160, device="cuda"))
+    v, _ = torch.linalg.qr(torch.randn(160, 160, device="cuda"))
+    s = torch.logspace(0, -1.5, 160, device="cuda")
+    out = ops.newton_schulz(u @ torch.diag(s) @ v)
+    got = torch.linalg.svdvals(out.cpu().double())
+    assert got.max() < 1.3 and got.min() > 0.6
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e-7, 1.0, 1e15, 1e30])
+@pytest.mark.parametrize("shape", [(48, 80), (140, 150)])
+def test_sizes_of_the_update(ops, shape, scale):
+    g = update(shape, seed=3) * scale
+    check(ops.newton_schulz(g), g, 5)
+
+
+def test_rows_of_very_different_size(ops):
+    g = update((96, 128), seed=4)
+    g[::3] *= 1e-5
+    g[1::3] = 0
+    out = ops.newton_schulz(g)
+    check(out, g, 5)
+    assert (out[1::3] == 0).all()
+
+
+def test_zeros_and_what_is_not_finite(ops):
+    g = torch.zeros(3, 40, 36, device="cuda")
+    g[1] = update((40, 36), seed=5)
+    g[2] = g[1]
+    g[2, 3, 4] = float("inf")
+    out = ops.newton_schulz(g)
+    assert (out[0] == 0).all() and out[2].isnan().all()
+    check(out[1], g[1], 5)
+    g[2, 3, 4] = float("nan")
+    assert ops.newton_schulz(g)[2].isnan().all()
+
+
+@pytest.mark.parametrize("shape", [(60, 90), (90, 60), (150, 200)])
+def test_strides_and_the_other_way_round(ops, shape):
+    g = update(shape, seed=6)
+    want = ops.newton_schulz(g)
+    big = torch.zeros(shape[0], 2 * shape[1], device="cuda")
+    big[:, ::2] = g
+    assert torch.equal(ops.newton_schulz(big[:, ::2]), want)
+    turned = ops.newton_schulz(g.t())
+    assert torch.equal(turned, want.t())
+
+
+@pytest.mark.parametrize("shape", [(30, 50), (140, 100)])
+def test_a_stack_has_the_bits_of_its_matrices(ops, shape):
+    g = update((5, *shape), seed=7)
+    out = ops.newton_schulz(g)
+    for i in range(5):
+        assert torch.equal(ops.newton_schulz(g[i]), out[i])
+
+
+def test_nothing(ops):
+    for shape in ((0, 4, 5), (4, 0), (0, 3)):
+        assert ops.newton_schulz(torch.empty(shape, device="cuda")).shape == shape
+
+
+@pytest.mark.parametrize("shape", [(2, 60, 40), (1, 200, 136)])
+def test_captured_and_replayed(ops, shape):
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    g = update(shape, seed=8)
+    ops.newton_schulz(g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.newton_schulz(g)
+    for _ in range(4):
+        g.normal_(generator=gen)
+        graph.replay()
+        got = y.clone()
+        assert torch.equal(got, ops.newton_schulz(g))
+
+
+def test_two_streams_at_once(ops):
+    gs = [update((180, 140), seed=s) for s in (1, 2)]
+    want = [ops.newton_schulz(g) for g in gs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in gs]
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.newton_schulz(gs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_refusals(ops):
+    g = torch.zeros(4, 4, device="cuda")
+    for bad in (lambda: ops.newton_schulz(g[0]), lambda: ops.newton_schulz(g, steps=0), lambda: ops.newton_schulz(g, steps=33), lambda: ops.newton_schulz(g, eps=-1.0),
+                lambda: ops.newton_schulz(g, eps=float("nan")), lambda: ops.newton_schulz(g, coefficients=(1.0, 2.0)),
+                lambda: ops.newton_schulz(g, coefficients=(1.0, 2.0, float("inf"))), lambda: ops.newton_schulz(torch.zeros(1, (1 << 20) + 1, device="cuda"))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: ops.newton_schulz(g.double()), lambda: ops.newton_schulz(g.cpu()), lambda: ops.newton_schulz([1.0])):
+        with pytest.raises(TypeError):
+            bad()
