@@ -241,6 +241,14 @@ __device__ __forceinline__ float lane_value(float v, int lane) { return __uint_a
 __device__ __forceinline__ float wave_max(float v) { return wave_butterfly(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float wave_sum(float v) { return wave_butterfly(v, [](float a, float b) { return a + b; }); }
 
+// What the lanes of a wave exchange through LDS without a barrier (its accesses are in order): the compiler keeps them there
+__device__ __forceinline__ void wave_fence() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#endif
+}
+
 // XCD-aware work-group numbering.  Consecutive work-group ids go round-robin over the 8 XCDs, each
 // with its own L2.  This maps id -> a logical index such that every XCD walks one contiguous
 // eighth of the logical range, so neighbouring tiles (which share operand panels) meet in one L2.

@@ -13,50 +13,184 @@
 namespace ppmlhip {
 namespace {
 
-constexpr int I8_MAX_K = 131071;
+constexpr int I8_MAX_K = 131071, I8_MAX_M = 1 << 22;
 
 // ------------------------------------------------------------------------------------------------------------ quantizer
-// A wave per row.  The row is read twice, the second time from the cache: bound by the first.
-struct I8Quantize {
+struct I8Rows {
     const void* x;
-    const float* scale_in;    // x holds int8 already: its rows are only laid out anew
-    int8_t* q;
-    float* scale;
-    int64_t rows, x_stride, q_stride;
-    int K, Kq;                // elements per row, and how many to write (zero from K on)
+    int type;                 // PPML_ELEM_*; I8: the rows are only laid out anew
+    int64_t stride;
+    const float* scale;       // I8: the rows' scales
+    int64_t rows;
+    int K;
 };
 
+// (the rows of any layout: four elements at the alignment of one)
+template <class T> struct Quad { typedef T Raw __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
+
+// the largest magnitude, NaN if there is one
+__device__ __forceinline__ float largest_of(float m, float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_elementwise_maximum(m, x);
+#else
+    return m + x;
+#endif
+}
 __device__ __forceinline__ float i8_scale(float largest) {
     // (infinite or NaN: the row's results are NaN by its scale; its values are written as zeros)
     return largest <= 3.402823466e38f ? largest * (1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
 }
-__device__ __forceinline__ int i8_value(float x, float scale) {
-    const float q = __builtin_rintf(x / scale);
-    return scale > 0.0f ? static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f)) : 0;
+__device__ __forceinline__ float i8_value(float x, float scale) {
+    return scale > 0.0f ? fminf(fmaxf(__builtin_rintf(x / scale), -127.0f), 127.0f) : 0.0f;
 }
-// the larger magnitude, NaN if either is one
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-    return a != a ? a : (b != b ? b : fmaxf(a, b));
+__device__ __forceinline__ uint32_t pack4(const float (&q)[4]) {
+    const uint32_t a = static_cast<uint32_t>(static_cast<int>(q[0])), b = static_cast<uint32_t>(static_cast<int>(q[1]));
+    const uint32_t c = static_cast<uint32_t>(static_cast<int>(q[2])), d = static_cast<uint32_t>(static_cast<int>(q[3]));
+    return (a & 255u) | (b & 255u) << 8 | (c & 255u) << 16 | d << 24;
+}
+// Four quantized values.  The quotient's rounding is the whole number next to x times the scale's reciprocal unless that product lies
+// within 2^-14 of a half: reciprocal, product and quotient are off by less than 127 (2^-23 + 2 * 2^-24) < 2^-15 together.  A division per
+// element costs a long row more than its way from memory (8192 rows of 4096 bf16 57 us with it, 27 without); one lane in 300 takes it.
+__device__ __forceinline__ uint32_t quantize4(const float (&x)[4], float scale, float inverse) {
+    float q[4], off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float t = x[e] * inverse;
+        q[e] = __builtin_rintf(t);
+        off = largest_of(off, __builtin_fabsf(t - q[e]));
+    }
+    // (a scale of zero, NaN, or too small for a reciprocal: `off` is NaN)
+    if (!(off <= 0.5f - 0x1p-14f)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = i8_value(x[e], scale);
+    }
+    return pack4(q);
 }
 
+// Elements k to k + 3 of a row of four or more, zeros behind its end, in two steps: the load, which is made whatever k is (the row's last four where
+// four from k on do not fit), and what becomes of it.  Loads under conditions, or with a use beside them, are waited for one after the other.
 template <class T>
-__global__ __launch_bounds__(256) void i8_quantize_kernel(const I8Quantize p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= p.rows) return;
-    const T* const x = static_cast<const T*>(p.x) + row * p.x_stride;
-    int8_t* const q = p.q + row * p.q_stride;
-    if constexpr (sizeof(T) == 1) {
-        for (int k = lane; k < p.Kq; k += 64) q[k] = k < p.K ? static_cast<int8_t>(x[k]) : static_cast<int8_t>(0);
-        return;
-    } else {
-        float largest = 0.0f;
-        for (int k = lane; k < p.K; k += 64) largest = max_or_nan(largest, __builtin_fabsf(to_f32(x[k])));
-        largest = wave_butterfly(largest, [](float a, float b) { return max_or_nan(a, b); });
-        const float scale = i8_scale(largest);
-        for (int k = lane; k < p.Kq; k += 64) q[k] = static_cast<int8_t>(k < p.K ? i8_value(to_f32(x[k]), scale) : 0);
-        if (lane == 0) p.scale[row] = scale;
+__device__ __forceinline__ typename Quad<T>::Raw fetch4(const T* row, int k, int K) {
+    return *reinterpret_cast<const typename Quad<T>::Raw*>(row + (k + 4 <= K ? k : K - 4));
+}
+template <class T>
+__device__ __forceinline__ void finish4(const typename Quad<T>::Raw& raw, int k, int K, float (&x)[4]) {
+    const int by = k + 4 <= K ? 0 : k + 4 - K;          // places that the loaded four lie too low
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = to_f32(static_cast<T>(raw[e]));
+    if (K & 3) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = by & 2 ? (e + 2 < 4 ? v[(e + 2) & 3] : 0.0f) : v[e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = by & 1 ? (e + 1 < 4 ? v[(e + 1) & 3] : 0.0f) : v[e];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = by < 4 ? v[e] : 0.0f;
+}
+
+// A wave's rows from `first` to `end`, of 4 to 256 R elements and at most G = 8 / R or 1 of them, kept in registers between the search for the largest and
+// the quantizing.  put(row, k, four values) for every k of a whole number of 256, and scale_is(row, scale).
+template <class T, int R, class Put, class ScaleIs>
+__device__ __forceinline__ void quantize_resident(const I8Rows& p, int64_t first, int64_t end, const Put& put, const ScaleIs& scale_is) {
+    constexpr int G = R >= 8 ? 1 : 8 / R;
+    const int lane = threadIdx.x & 63;
+    if (first >= end) return;
+    typename Quad<T>::Raw raw[G][R];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const T* const row = static_cast<const T*>(p.x) + (first + g < end ? first + g : end - 1) * p.stride;
+#pragma unroll
+        for (int i = 0; i < R; ++i) raw[g][i] = fetch4<T>(row, 4 * (lane + 64 * i), p.K);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        if (first + g >= end) break;
+        float x[R][4], largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) finish4<T>(raw[g][i], 4 * (lane + 64 * i), p.K, x[i]);
+        if constexpr (sizeof(T) == 1) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) put(first + g, 4 * (lane + 64 * i), pack4(x[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
+            largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
+            const float scale = i8_scale(largest), inverse = __builtin_amdgcn_rcpf(scale);
+#pragma unroll
+            for (int i = 0; i < R; ++i) put(first + g, 4 * (lane + 64 * i), quantize4(x[i], scale, inverse));
+            scale_is(first + g, scale);
+        }
+    }
+}
+// Longer rows are read twice, the second time from the cache; rows of fewer than four elements as well
+template <class T, class Put, class ScaleIs>
+__device__ __forceinline__ void quantize_twice(const I8Rows& p, int64_t first, int64_t end, const Put& put, const ScaleIs& scale_is) {
+    const int lane = threadIdx.x & 63;
+    const auto load = [&](const T* row, int k, float (&x)[4]) {
+        if (p.K >= 4) finish4<T>(fetch4<T>(row, k, p.K), k, p.K, x);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = k + e < p.K ? to_f32(row[k + e]) : 0.0f;
+    };
+    for (int64_t r = first; r < end; ++r) {
+        const T* const row = static_cast<const T*>(p.x) + r * p.stride;
+        float scale = 0.0f, inverse = 0.0f;
+        if constexpr (sizeof(T) > 1) {
+            float largest = 0.0f;
+            const auto meet = [&](const float (&x)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[e]));
+            };
+            int k = 4 * lane;
+            for (; k + 2048 <= p.K; k += 2048) {
+                typename Quad<T>::Raw raw[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) raw[u] = fetch4<T>(row, k + 256 * u, p.K);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    float x[4];
+                    finish4<T>(raw[u], k + 256 * u, p.K, x);
+                    meet(x);
+                }
+            }
+            for (; k < p.K; k += 256) {
+                float x[4];
+                load(row, k, x);
+                meet(x);
+            }
+            largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
+            scale = i8_scale(largest);
+            inverse = __builtin_amdgcn_rcpf(scale);
+            scale_is(r, scale);
+        }
+        for (int k = 4 * lane; k < (p.K + 255) / 256 * 256; k += 256) {
+            float x[4];
+            load(row, k, x);
+            put(r, k, sizeof(T) == 1 ? pack4(x) : quantize4(x, scale, inverse));
+        }
+    }
+}
+
+// `put` stores four values at k: all of them below the row's end, which is K or that up to a multiple of 128
+__device__ __forceinline__ void put_row(int8_t* row, int k, int end, uint32_t v) {
+    typedef uint32_t any32 __attribute__((aligned(1)));
+    if (k + 4 <= end) *reinterpret_cast<any32*>(row + k) = v;
+    else
+        for (int e = 0; e < 4 && k + e < end; ++e) row[k + e] = static_cast<int8_t>(v >> 8 * e);
+}
+
+// A wave per row (R = 0: rows of any length)
+template <class T, int R>
+__global__ __launch_bounds__(256) void i8_quantize_kernel(const I8Rows p, int8_t* q, int64_t q_stride, int q_end, float* scales) {
+    constexpr int G = R == 0 || R >= 8 ? 1 : 8 / R;
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * G, end = first + G < p.rows ? first + G : p.rows;
+    const auto put = [&](int64_t row, int k, uint32_t v) { put_row(q + row * q_stride, k, q_end, v); };
+    const auto scale_is = [&](int64_t row, float scale) { if ((threadIdx.x & 63) == 0) scales[row] = scale; };
+    if constexpr (R == 0) quantize_twice<T>(p, first, end, put, scale_is);
+    else quantize_resident<T, R>(p, first, end, put, scale_is);
 }
 
 // ------------------------------------------------------------------------------------------------------------ product
@@ -67,59 +201,379 @@ struct I8Product {
     int stages, tiles_w, tiles_x;
 };
 
-template <class T, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(WM * WN * 64) void i8_product_kernel(const I8Product p) {
-    typedef TileLoop<StepI8, WM, WN, TM, TN> Loop;
-    const int t = xcd_contiguous_index(blockIdx.x, p.tiles_w * p.tiles_x);
-    const int m0 = (t % p.tiles_w) * Loop::BM, n0 = (t / p.tiles_w) * Loop::BN;
-    v4i acc[TM][TN];
-    Loop::run(p.w, p.x, m0, n0, p.stages, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int mw = m0 + wave / WN * TM * 16 + (lane >> 4) * 4, nw = n0 + wave % WN * TN * 16 + (lane & 15);
-    const int M = p.w.rows;
+// What a lane multiplies and adds to its channels of a wave's 16 TM from mw on
+template <class T, int TM>
+struct Channels {
+    static constexpr int V = 16 / sizeof(T), ACROSS = TM * 16 / V;      // channels per lane, lanes per token
+    static_assert(64 % ACROSS == 0, "a lane keeps its channels");
+    float scale[V], bias[V];
+    int m;
+    __device__ __forceinline__ Channels(const I8Product& p, int mw) {
+        m = mw + (threadIdx.x & 63) % ACROSS * V;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        float ws[4], b[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int m = mw + 16 * i + r < M ? mw + 16 * i + r : M - 1;
-            ws[r] = p.w_scale[m];
-            b[r] = p.bias ? p.bias[m] : 0.0f;
+        for (int e = 0; e < V; ++e) {
+            const int at = m + e < p.w.rows ? m + e : p.w.rows - 1;
+            scale[e] = p.w_scale[at];
+            bias[e] = p.bias ? p.bias[at] : 0.0f;
         }
+    }
+};
+
+// The outputs of a wave: TM x TN tiles of its channels and the tokens from nw on.  Sixteen tokens at a time go through LDS (16 (16 TM + 4)
+// floats), where a lane's four consecutive channels become whole lines of the output: stored as the matrix instruction leaves
+// them, a token's channels went out in pieces of 16 bytes (f32) and 8 (the alignment's projection 60 us instead of 22).
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+constexpr uint32_t OUTSIDE_ROWS = 0xfffffff0u;           // no resource here is that long
+template <bool VEC, class T, int TM, int TN>
+__device__ __forceinline__ void store_tokens(const I8Product& p, const Channels<T, TM>& ch, float* lds, int nw, const v4i (&acc)[TM][TN], const float* x_scale) {
+    constexpr int PITCH = TM * 16 + 4;                  // floats: the rows of sixteen lanes' pieces in banks of their own
+    constexpr int V = Channels<T, TM>::V, ACROSS = Channels<T, TM>::ACROSS;
+    const int lane = threadIdx.x & 63, M = p.w.rows, c = lane % ACROSS * V, m = ch.m;
+    // (stores outside, by their offsets, are none: without a condition around them the compiler knows how many there are, and waits for loads
+    // that were requested before them without waiting for the stores)
+    const int64_t left = (static_cast<int64_t>(p.x.rows) - nw) * M * sizeof(T), most = static_cast<int64_t>(TN * 16) * M * sizeof(T);
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(static_cast<T*>(p.y) + static_cast<int64_t>(nw) * M, 0,
+                                                                          static_cast<int>(left < 0 ? 0 : left < most ? left : most), 0x00020000);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int n = nw + 16 * j;
-            if (n >= p.x.rows) continue;
-            const float xs = p.x_scale[n];
-            T* const y = static_cast<T*>(p.y) + static_cast<int64_t>(n) * M;
+    for (int j = 0; j < TN; ++j) {
+        const float xs = x_scale[16 * j + (lane & 15)];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float v = static_cast<float>(acc[i][j][r]) * xs * ws[r];
-                if (mw + 16 * i + r < M) y[mw + 16 * i + r] = from_f32<T>(p.bias ? v + b[r] : v);
+        for (int i = 0; i < TM; ++i) {
+            v4f v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(acc[i][j][r]) * xs;
+            *reinterpret_cast<v4f*>(lds + (lane & 15) * PITCH + 16 * i + (lane >> 4) * 4) = v;
+        }
+        wave_fence();
+#pragma unroll
+        for (int k = 0; k < 16 * ACROSS / 64; ++k) {
+            const int token = (k * 64 + lane) / ACROSS;
+            const uint32_t at = static_cast<uint32_t>((16 * j + token) * static_cast<int64_t>(M) + m) * static_cast<uint32_t>(sizeof(T));
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) *reinterpret_cast<v4f*>(v + e) = *reinterpret_cast<const v4f*>(lds + token * PITCH + c + e);
+            typename Elements<T, V>::Raw raw;
+#pragma unroll
+            for (int e = 0; e < V; ++e) raw[e] = from_f32<T>(p.bias ? v[e] * ch.scale[e] + ch.bias[e] : v[e] * ch.scale[e]);
+            if (VEC) {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, raw), rsrc, m < M ? at : OUTSIDE_ROWS, 0, 0);
+            } else if (nw + 16 * j + token < p.x.rows) {
+                // (rows of any length: the same stores at the alignment of an element, but for the last few channels)
+                typedef T any __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+                T* const to = static_cast<T*>(p.y) + (static_cast<int64_t>(nw) + 16 * j + token) * M + m;
+                if (m + V <= M) *reinterpret_cast<any*>(to) = raw;
+                else
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (m + e < M) to[e] = raw[e];
             }
         }
+        wave_fence();
+    }
+}
+// whether outputs leave sixteen bytes at a time
+template <class T>
+__device__ __forceinline__ bool whole_stores(const I8Product& p) { return p.w.rows % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0; }
+
+template <class T, class Loop>
+__global__ __launch_bounds__(Loop::THREADS, 2) void i8_product_kernel(const I8Product p) {
+    constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN, PITCH = TM * 16 + 4;
+    __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
+    __shared__ float x_scale[Loop::BN];
+    const int t = xcd_contiguous_index(blockIdx.x, p.tiles_w * p.tiles_x);
+    const int m0 = (t % p.tiles_w) * Loop::BM, n0 = (t / p.tiles_w) * Loop::BN;
+    for (int i = threadIdx.x; i < Loop::BN; i += Loop::THREADS) x_scale[i] = p.x_scale[n0 + i < p.x.rows ? n0 + i : p.x.rows - 1];
+    v4i acc[TM][TN];
+    Loop::run(p.w, p.x, m0, n0, p.stages, even, odd, acc);
+    const int wave = threadIdx.x >> 6, nw = wave % WN * TN * 16;
+    static_assert(Loop::WAVES / 2 * 16 * PITCH * 4 <= Loop::STAGE, "half of the waves' sixteen tokens fit a stage");
+    __syncthreads();                                    // every wave has read its last stage
+    float* const lds = reinterpret_cast<float*>(wave & 1 ? odd : even) + (wave >> 1) * 16 * PITCH;
+    const Channels<T, TM> ch(p, m0 + wave / WN * TM * 16);
+    if (whole_stores<T>(p)) store_tokens<true>(p, ch, lds, n0 + nw, acc, x_scale + nw);
+    else                    store_tokens<false>(p, ch, lds, n0 + nw, acc, x_scale + nw);
+}
+
+// Few tokens (at most 16): what counts is the weight's way from memory.  A work-group takes 16 channels, its waves every WAVES-th stage of
+// k, all requested before the first product.  The tokens are quantized in every work-group, into LDS, where they are few enough for that
+// to cost less than a launch of its own.
+constexpr int I8_FEW_WAVES = 8, I8_FEW_PART = 2048;     // elements of a row that a wave quantizes at most
+__host__ __device__ constexpr int few_share(int tokens) { return tokens <= 1 ? 8 : tokens <= 2 ? 4 : tokens <= 4 ? 2 : 1; }      // waves per token
+
+template <class T>
+__global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Product p, const I8Rows rows) {
+    constexpr int DEEP = 8, WAVES = I8_FEW_WAVES;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_q[];      // [tokens][row + 16], behind it the sums
+    __shared__ float x_scale[16];
+    __shared__ int sums[WAVES][16][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tokens = p.x.rows, m0 = blockIdx.x * 16, row_bytes = p.stages * TILE_K, pitch = row_bytes + 16;
+    const RowBytes W = p.w;
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(W.base + m0 * W.stride), 0, 0x7fffffff, 0x00020000);
+    const int last = W.rows - 1 - m0, r = (lane & 15) < last ? lane & 15 : last;
+    const uint32_t from = static_cast<uint32_t>(r * W.stride) + (lane >> 4) * 16u;
+    v4i a[DEEP][2];
+    const auto request = [&](int first) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int stage = first + d * WAVES < p.stages ? first + d * WAVES : p.stages - 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) a[d][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, from, stage * TILE_K + h * 64, 0));
+        }
+    };
+    request(wave);
+    const auto put = [&](int64_t row, int k, uint32_t v) { if (k < row_bytes) *reinterpret_cast<uint32_t*>(lds_q + row * pitch + k) = v; };
+    // a token's row goes to `share` waves; R quads of every lane hold its part of at most 256 R elements
+    constexpr int R = I8_FEW_PART / 256;
+    const int share = few_share(tokens);
+    const auto each = [&](auto zero) {
+        typedef decltype(zero) E;
+        const int part = wave % share, piece = (row_bytes / 4 + 64 * share - 1) / (64 * share) * 256;      // elements of a wave's part
+        for (int first = 0; first < tokens; first += WAVES / share) {
+            const int t = first + wave / share, k0 = part * piece + 4 * lane;
+            const E* const row = static_cast<const E*>(rows.x) + static_cast<int64_t>(t < tokens ? t : tokens - 1) * rows.stride;
+            typename Quad<E>::Raw raw[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) raw[i] = fetch4<E>(row, 256 * i < piece ? k0 + 256 * i : rows.K, rows.K);
+            float x[R][4], largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < R; ++i) finish4<E>(raw[i], 256 * i < piece ? k0 + 256 * i : rows.K, rows.K, x[i]);
+            float scale = 0.0f, inverse = 0.0f;
+            if constexpr (sizeof(E) > 1) {
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
+                largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
+                if (share > 1) {                        // (the loop is made once)
+                    if (lane == 0) x_scale[wave] = largest;
+                    __syncthreads();
+                    largest = 0.0f;
+                    for (int w = 0; w < share; ++w) largest = largest_of(largest, x_scale[wave - part + w]);
+                    __syncthreads();
+                }
+                scale = i8_scale(largest);
+                inverse = __builtin_amdgcn_rcpf(scale);
+                if (lane == 0 && part == 0 && t < tokens) x_scale[t] = scale;
+            }
+            if (t < tokens) {
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+                    if (256 * i < piece) put(t, k0 + 256 * i, sizeof(E) == 1 ? pack4(x[i]) : quantize4(x[i], scale, inverse));
+            }
+        }
+    };
+    switch (rows.type) {
+        case PPML_ELEM_F32:  each(0.0f); break;
+        case PPML_ELEM_F16:  each(static_cast<_Float16>(0)); break;
+        case PPML_ELEM_BF16: each(static_cast<__bf16>(0)); break;
+        default:             each(static_cast<int8_t>(0)); break;
+    }
+    if (rows.type == PPML_ELEM_I8 && static_cast<int>(threadIdx.x) < tokens) x_scale[threadIdx.x] = rows.scale[threadIdx.x];
+    __syncthreads();
+    const uint8_t* const token = lds_q + ((lane & 15) < tokens ? lane & 15 : tokens - 1) * pitch + (lane >> 4) * 16;
+    v4i acc{};
+    for (int first = wave; first < p.stages; first += WAVES * DEEP) {
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const int stage = first + d * WAVES;
+            if (stage < p.stages) {
+                const v4i b[2] = {*reinterpret_cast<const v4i*>(token + stage * TILE_K), *reinterpret_cast<const v4i*>(token + stage * TILE_K + 64)};
+                StepI8::step<0>(a[d], b, acc);
+                StepI8::step<1>(a[d], b, acc);
+            }
+        }
+        if (first + WAVES * DEEP < p.stages) request(first + WAVES * DEEP);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[wave][lane & 15][(lane >> 4) * 4 + e] = acc[e];
+    __syncthreads();
+    const int n = threadIdx.x >> 4, m = m0 + (threadIdx.x & 15);
+    if (n >= tokens || m >= W.rows) return;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += sums[w][n][threadIdx.x & 15];
+    const float v = static_cast<float>(sum) * x_scale[n] * p.w_scale[m];
+    static_cast<T*>(p.y)[static_cast<int64_t>(n) * W.rows + m] = from_f32<T>(p.bias ? v + p.bias[m] : v);
+}
+
+// Short rows (at most 128 S elements) and more tokens: bound by the way of x and y from and to memory.  A wave keeps its 64 channels of the weight
+// in registers, a work-group stays and takes every gridDim.x-th group of 4 WAVES tokens: their rows, requested a group ahead, are quantized
+// into LDS by all its waves, and every wave multiplies them with its channels.  One launch, x read once (once per part of 64 WAVES channels).
+// A wave quantizes four rows at a time, sixteen lanes each: the search for the largest then takes four steps for four rows (a row
+// at a time by 64 lanes, six steps each, the alignment's projection was bound by it: 39 us).
+template <class T, bool VEC, int S, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void i8_stay_kernel(const I8Product p, const I8Rows rows) {
+    constexpr int TM = 4, TN = WAVES / 4, TOKENS = TN * 16, PITCH = TM * 16 + 4, ROW = S * TILE_K, LDS_ROW = ROW + 16;
+    constexpr int QUADS = ROW / 64;                     // of a row per lane
+    __shared__ __attribute__((aligned(16))) float out_all[WAVES][16 * PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t lds_q[2][TOKENS * LDS_ROW];
+    __shared__ float x_scale[2][TOKENS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tokens = p.x.rows, groups = (tokens + TOKENS - 1) / TOKENS;
+    const int mw = (blockIdx.y * WAVES + wave) * 64;
+    const RowBytes W = p.w;
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(W.base), 0, static_cast<int>(W.rows * W.stride), 0x00020000);
+    v4i a[S][TM][2];
+    {
+        // (rows behind the last one lie outside the resource and read as nothing)
+        const uint32_t from = static_cast<uint32_t>((mw + (lane & 15)) * W.stride) + (lane >> 4) * 16u;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    a[s][i][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, from + static_cast<uint32_t>(16 * i * W.stride) + s * TILE_K + h * 64, 0, 0));
+    }
+    const Channels<T, TM> ch(p, mw);
+    float* const out = out_all[wave];
+    const int mine = wave * 4 + (lane >> 4), k0 = (lane & 15) * 4;      // the row of the group, and the first element, that this lane quantizes
+    // (what is loaded once is here before the loop begins: waits for it inside would be waits for the rows requested there as well)
+    __builtin_amdgcn_s_waitcnt(0x0f70);                 // vmcnt(0)
+    const auto run = [&](auto zero) {
+        typedef decltype(zero) E;
+        typename Quad<E>::Raw raw[QUADS];
+        float given = 0.0f;
+        // (without a condition: past the last token the last one)
+        const auto request = [&](int group) {
+            const int64_t t = static_cast<int64_t>(group) * TOKENS + mine, at = t < tokens ? t : tokens - 1;
+            const E* const row = static_cast<const E*>(rows.x) + at * rows.stride;
+#pragma unroll
+            for (int i = 0; i < QUADS; ++i) raw[i] = fetch4<E>(row, k0 + 64 * i, rows.K);
+            if constexpr (sizeof(E) == 1) given = rows.scale[at];
+        };
+        int group = blockIdx.x, side = 0;
+        request(group);
+        for (; group < groups; group += gridDim.x, side ^= 1) {
+            float x[QUADS][4], scale = given, inverse = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QUADS; ++i) finish4<E>(raw[i], k0 + 64 * i, rows.K, x[i]);
+            if constexpr (sizeof(E) > 1) {
+                float largest = 0.0f;
+#pragma unroll
+                for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
+                scale = i8_scale(row16_butterfly(largest, [](float u, float v) { return largest_of(u, v); }));
+                inverse = __builtin_amdgcn_rcpf(scale);
+            }
+#pragma unroll
+            for (int i = 0; i < QUADS; ++i)
+                *reinterpret_cast<uint32_t*>(lds_q[side] + mine * LDS_ROW + k0 + 64 * i) = sizeof(E) == 1 ? pack4(x[i]) : quantize4(x[i], scale, inverse);
+            if ((lane & 15) == 0) x_scale[side][mine] = scale;
+            request(group + gridDim.x);
+            __syncthreads();                            // (the group before this one was read before the last one of these)
+            v4i acc[TM][TN];
+#pragma unroll
+            for (int u = 0; u < TM; ++u)
+#pragma unroll
+                for (int v = 0; v < TN; ++v) acc[u][v] = v4i{};
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                v4i b[TN][2];
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        b[j][h] = *reinterpret_cast<const v4i*>(lds_q[side] + (16 * j + (lane & 15)) * LDS_ROW + s * TILE_K + h * 64 + (lane >> 4) * 16);
+                step_tiles<StepI8>(a[s], b, acc);
+            }
+            store_tokens<VEC>(p, ch, out, group * TOKENS, acc, x_scale[side]);
+        }
+    };
+    switch (rows.type) {
+        case PPML_ELEM_F32:  run(0.0f); break;
+        case PPML_ELEM_F16:  run(static_cast<_Float16>(0)); break;
+        case PPML_ELEM_BF16: run(static_cast<__bf16>(0)); break;
+        default:             run(static_cast<int8_t>(0)); break;
     }
 }
 
 int64_t i8_row_bytes(int64_t K) { return (K + TILE_K - 1) / TILE_K * TILE_K; }
 
-int launch_quantize(const I8Quantize& p, int type, hipStream_t stream, const char* what) {
-    const int64_t blocks = (p.rows + 3) / 4;
-    if (blocks > 0x7fffffff) { set_error("%s: too many rows", what); return RC_BAD_ARGS; }
-    const dim3 grid(static_cast<unsigned>(blocks)), block(256);
-    switch (type) {
-        case PPML_ELEM_F32:  hipLaunchKernelGGL((i8_quantize_kernel<float>), grid, block, 0, stream, p); break;
-        case PPML_ELEM_F16:  hipLaunchKernelGGL((i8_quantize_kernel<_Float16>), grid, block, 0, stream, p); break;
-        case PPML_ELEM_BF16: hipLaunchKernelGGL((i8_quantize_kernel<__bf16>), grid, block, 0, stream, p); break;
-        default:             hipLaunchKernelGGL((i8_quantize_kernel<int8_t>), grid, block, 0, stream, p); break;
+template <class T>
+void launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, float* scale, int64_t waves, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), block(256);
+    const int pieces = (p.K + 255) / 256;
+    if (p.K < 4 || pieces > 16) hipLaunchKernelGGL((i8_quantize_kernel<T, 0>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+    else if (pieces <= 1)  hipLaunchKernelGGL((i8_quantize_kernel<T, 1>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+    else if (pieces <= 2)  hipLaunchKernelGGL((i8_quantize_kernel<T, 2>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+    else if (pieces <= 4)  hipLaunchKernelGGL((i8_quantize_kernel<T, 4>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+    else if (pieces <= 8)  hipLaunchKernelGGL((i8_quantize_kernel<T, 8>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+    else                   hipLaunchKernelGGL((i8_quantize_kernel<T, 16>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+}
+int launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, float* scale, hipStream_t stream, const char* what) {
+    const int pieces = (p.K + 255) / 256, per_wave = p.K < 4 ? 1 : pieces <= 1 ? 8 : pieces <= 2 ? 4 : pieces <= 4 ? 2 : 1;
+    const int64_t waves = (p.rows + per_wave - 1) / per_wave;
+    if (waves > 4ll * 0x7fffffff) { set_error("%s: too many rows", what); return RC_BAD_ARGS; }
+    switch (p.type) {
+        case PPML_ELEM_F32:  launch_quantize<float>(p, q, q_stride, q_end, scale, waves, stream); break;
+        case PPML_ELEM_F16:  launch_quantize<_Float16>(p, q, q_stride, q_end, scale, waves, stream); break;
+        case PPML_ELEM_BF16: launch_quantize<__bf16>(p, q, q_stride, q_end, scale, waves, stream); break;
+        default:             launch_quantize<int8_t>(p, q, q_stride, q_end, scale, waves, stream); break;
     }
     return check_launch(what);
 }
 
+template <class T, class Loop>
+int launch_tiles(I8Product p, hipStream_t stream) {
+    p.tiles_w = (p.w.rows + Loop::BM - 1) / Loop::BM;
+    p.tiles_x = (p.x.rows + Loop::BN - 1) / Loop::BN;
+    if (static_cast<int64_t>(p.tiles_w) * p.tiles_x > 0x7fffffff) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
+    hipLaunchKernelGGL((i8_product_kernel<T, Loop>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x)), dim3(Loop::THREADS), 0, stream, p);
+    return check_launch("mul_mat_i8_hip");
+}
+
+template <class T, bool VEC, int S, int WAVES>
+void launch_stay_waves(const I8Product& p, const I8Rows& rows, hipStream_t stream) {
+    const int parts = (p.w.rows + 64 * WAVES - 1) / (64 * WAVES), groups = (p.x.rows + 4 * WAVES - 1) / (4 * WAVES);
+    // measured, 26368 tokens of 256: onto 256 channels 256 / 512 / 768 / 1024 work-groups of four waves 15.5 / 14.5 / 15.7 / 18.9 us (eight waves
+    // 16.1), onto 768 work-groups of eight waves 25.6 / 30.0 / 33.5 / 36.9 (four waves 27.3 at best, twelve 32.5)
+    int wgs = (WAVES == 4 ? 2 : 1) * device_cu_count() / parts;
+    if (wgs < 1) wgs = 1;
+    if (wgs > groups) wgs = groups;
+    hipLaunchKernelGGL((i8_stay_kernel<T, VEC, S, WAVES>), dim3(wgs, parts), dim3(64 * WAVES), 0, stream, p, rows);
+}
+template <class T, int S>
+void launch_stay(const I8Product& p, const I8Rows& rows, hipStream_t stream) {
+    const bool vec = p.w.rows % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+    const int blocks = (p.w.rows + 63) / 64;
+    if (blocks <= 4) vec ? launch_stay_waves<T, true, S, 4>(p, rows, stream) : launch_stay_waves<T, false, S, 4>(p, rows, stream);
+    else             vec ? launch_stay_waves<T, true, S, 8>(p, rows, stream) : launch_stay_waves<T, false, S, 8>(p, rows, stream);
+}
+
+// How a product is made
+enum I8Form { I8_FEW, I8_STAY, I8_TILES };
+constexpr int I8_FEW_LDS = 40 << 10, I8_STAY_STAGES = 4;
+I8Form i8_form(int M, int N, int K) {
+    const int64_t row = i8_row_bytes(K);
+    if (K < 4) return I8_TILES;                         // (the rows are fetched four elements at a time)
+    if (N <= 16 && row <= I8_FEW_PART * few_share(N) && N * (row + 16) <= I8_FEW_LDS) return I8_FEW;
+    if (row <= I8_STAY_STAGES * TILE_K && (M + 511) * row < 0x7fffffff) return I8_STAY;
+    return I8_TILES;
+}
+
 template <class T>
-void launch_product(const I8Product& p, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.tiles_w * p.tiles_x));
-    hipLaunchKernelGGL((i8_product_kernel<T, 2, 2, 4, 4>), grid, dim3(256), 0, stream, p);
+int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* scale, I8Form form, hipStream_t stream) {
+    const int row = p.stages * TILE_K;
+    if (form == I8_FEW) {
+        const dim3 grid(static_cast<unsigned>((p.w.rows + 15) / 16));
+        const size_t lds = static_cast<size_t>(p.x.rows) * (row + 16);
+        hipLaunchKernelGGL((i8_few_kernel<T>), grid, dim3(I8_FEW_WAVES * 64), lds, stream, p, rows);
+        return check_launch("mul_mat_i8_hip");
+    }
+    if (form == I8_STAY) {
+        if (p.stages == 1)      launch_stay<T, 1>(p, rows, stream);
+        else if (p.stages == 2) launch_stay<T, 2>(p, rows, stream);
+        else                    launch_stay<T, 4>(p, rows, stream);
+        return check_launch("mul_mat_i8_hip");
+    }
+    const int rc = launch_quantize(rows, q, row, row, scale, stream, "mul_mat_i8_hip");
+    if (rc != RC_OK) return rc;
+    const int64_t tiles256 = static_cast<int64_t>((p.w.rows + 255) / 256) * ((p.x.rows + 255) / 256);
+    if (tiles256 >= device_cu_count()) return launch_tiles<T, TilePingPong<StepI8>>(p, stream);
+    return launch_tiles<T, TileLoop<StepI8, 2, 2, 4, 4>>(p, stream);
 }
 
 bool float_type(int type) { return type == PPML_ELEM_F32 || type == PPML_ELEM_F16 || type == PPML_ELEM_BF16; }
@@ -131,13 +585,12 @@ using namespace ppmlhip;
 
 extern "C" int quantize_rows_i8_hip(const void* x, int type, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int64_t rows, int K,
                                     ppml_hip_stream_t stream) {
-    const int64_t Kq = q_stride == i8_row_bytes(K) ? q_stride : K;
     if (!x || !q || !float_type(type) || !scale || rows <= 0 || K <= 0 || K > I8_MAX_K || x_stride < K || q_stride < K) {
         set_error("quantize_rows_i8_hip: bad arguments (rows=%lld K=%d type=%d)", (long long)rows, K, type);
         return RC_BAD_ARGS;
     }
-    return launch_quantize(I8Quantize{x, nullptr, q, scale, rows, x_stride, q_stride, K, static_cast<int>(Kq)}, type, static_cast<hipStream_t>(stream),
-                           "quantize_rows_i8_hip");
+    const int end = q_stride == i8_row_bytes(K) ? static_cast<int>(q_stride) : K;
+    return launch_quantize(I8Rows{x, type, x_stride, nullptr, rows, K}, q, q_stride, end, scale, static_cast<hipStream_t>(stream), "quantize_rows_i8_hip");
 }
 
 extern "C" size_t i8_weight_row_bytes_hip(int K) { return K > 0 && K <= I8_MAX_K ? static_cast<size_t>(i8_row_bytes(K)) : 0; }
@@ -148,7 +601,7 @@ extern "C" int i8_weight_pack_hip(const int8_t* w, int64_t w_stride, int M, int 
         return RC_BAD_ARGS;
     }
     const int64_t row = i8_row_bytes(K);
-    return launch_quantize(I8Quantize{w, nullptr, packed, nullptr, M, w_stride, row, K, static_cast<int>(row)}, PPML_ELEM_I8, static_cast<hipStream_t>(stream),
+    return launch_quantize(I8Rows{w, PPML_ELEM_I8, w_stride, nullptr, M, K}, packed, row, static_cast<int>(row), nullptr, static_cast<hipStream_t>(stream),
                            "i8_weight_pack_hip");
 }
 
@@ -160,7 +613,7 @@ extern "C" size_t mul_mat_i8_workspace_hip(int N, int K) {
 extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const void* x, int x_type, int64_t x_stride, const float* x_scale, const float* bias,
                               void* y, int y_type, int M, int N, int K, void* workspace, size_t workspace_bytes, ppml_hip_stream_t stream_) {
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
-    if (!packed || !w_scale || !x || !y || M <= 0 || N <= 0 || K <= 0 || K > I8_MAX_K || x_stride < K || !float_type(y_type) ||
+    if (!packed || !w_scale || !x || !y || M <= 0 || M > I8_MAX_M || N <= 0 || K <= 0 || K > I8_MAX_K || x_stride < K || !float_type(y_type) ||
         (x_type == PPML_ELEM_I8 ? !x_scale : !float_type(x_type)) || (reinterpret_cast<uintptr_t>(packed) & 15) != 0) {
         set_error("mul_mat_i8_hip: bad arguments (M=%d N=%d K=%d x_type=%d y_type=%d)", M, N, K, x_type, y_type);
         return RC_BAD_ARGS;
@@ -173,8 +626,6 @@ extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const 
     const int64_t row = i8_row_bytes(K);
     int8_t* const q = static_cast<int8_t*>(workspace);
     float* const scale = reinterpret_cast<float*>(q + static_cast<int64_t>(N) * row);
-    const int rc = launch_quantize(I8Quantize{x, x_scale, q, scale, N, x_stride, row, K, static_cast<int>(row)}, x_type, stream, "mul_mat_i8_hip");
-    if (rc != RC_OK) return rc;
     I8Product p{};
     p.w = RowBytes{reinterpret_cast<const uint8_t*>(packed), row, M};
     p.x = RowBytes{reinterpret_cast<const uint8_t*>(q), row, N};
@@ -183,13 +634,11 @@ extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const 
     p.bias = bias;
     p.y = y;
     p.stages = static_cast<int>(row / TILE_K);
-    p.tiles_w = (M + 127) / 128;
-    p.tiles_x = (N + 127) / 128;
-    if (static_cast<int64_t>(p.tiles_w) * p.tiles_x > 0x7fffffff) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
+    const I8Rows rows{x, x_type, x_stride, x_scale, N, K};
+    const I8Form form = i8_form(M, N, K);
     switch (y_type) {
-        case PPML_ELEM_F32:  launch_product<float>(p, stream); break;
-        case PPML_ELEM_F16:  launch_product<_Float16>(p, stream); break;
-        default:             launch_product<__bf16>(p, stream); break;
+        case PPML_ELEM_F32:  return launch_product<float>(p, rows, q, scale, form, stream);
+        case PPML_ELEM_F16:  return launch_product<_Float16>(p, rows, q, scale, form, stream);
+        default:             return launch_product<__bf16>(p, rows, q, scale, form, stream);
     }
-    return check_launch("mul_mat_i8_hip");
 }

@@ -19,7 +19,7 @@
 namespace ppmlhip {
 namespace {
 
-constexpr int NS_MOST_STEPS = 32, NS_NORM_BLOCKS = 64;
+constexpr int NS_MOST_STEPS = 32, NS_NORM_BLOCKS = 1024;
 constexpr int64_t NS_MOST_SIDE = 1 << 20;
 
 // (per matrix) what the launches multiply by: sums of products and the matrix that is added, to the next operand's scale
@@ -67,34 +67,66 @@ __device__ int operand_exponent(double bound) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ norm
+// Each work-group a run of the matrix, its partial sum in 64 bits: no update is so large or so small that its norm leaves the range
 template <class T>
-__global__ __launch_bounds__(256) void ns_norm_kernel(const T* g, int64_t count, double* partial) {
-    __shared__ double lds[256];
+__global__ __launch_bounds__(256) void ns_norm_kernel(const T* g, int64_t count, double* partial, int vec) {
+    __shared__ double lds[4];
     const T* const x = g + blockIdx.y * count;
     double sum = 0.0;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const double v = static_cast<double>(to_f32(x[i]));
-        sum = fma(v, v, sum);
+    const auto add = [&](float v) { sum = fma(static_cast<double>(v), static_cast<double>(v), sum); };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256, first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (vec) {
+        int64_t i = first;
+        for (; i + 3 * step < count / 4; i += 4 * step) {
+            float v[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_f32<T, 4>(x + 4 * (i + u * step), v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) add(v[u][e]);
+        }
+        for (; i < count / 4; i += step) {
+            float v[4];
+            load_f32<T, 4>(x + 4 * i, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add(v[e]);
+        }
+    } else {
+        for (int64_t i = first; i < count; i += step) add(to_f32(x[i]));
     }
-    lds[threadIdx.x] = sum;
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
     __syncthreads();
-    for (int step = 128; step > 0; step >>= 1) {
-        if (static_cast<int>(threadIdx.x) < step) lds[threadIdx.x] += lds[threadIdx.x + step];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) partial[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = lds[0];
+    if (threadIdx.x == 0) partial[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
 // ------------------------------------------------------------------------------------------------------------ operands
-// Where an element lies in an operand: its upper half (the lower one 64 bytes behind)
+// Where a group of 32 elements lies in an operand: their upper halves, the lower ones 64 bytes behind
 __device__ __forceinline__ int64_t operand_at(int64_t row, int64_t stride, int k) { return row * stride + (k >> 5) * 128 + (k & 31) * 2; }
-__device__ __forceinline__ float operand_value(const uint8_t* at) {
-    return static_cast<float>(*reinterpret_cast<const _Float16*>(at)) + static_cast<float>(*reinterpret_cast<const _Float16*>(at + 64));
+
+// Sixteen consecutive elements of a group
+__device__ __forceinline__ void put_operand(uint8_t* at, const float (&x)[16]) {
+#pragma unroll
+    for (int o = 0; o < 16; o += 8) {
+        v8h h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[e] = static_cast<_Float16>(x[o + e]);
+            l[e] = static_cast<_Float16>(x[o + e] - static_cast<float>(h[e]));
+        }
+        *reinterpret_cast<v8h*>(at + 2 * o) = h;
+        *reinterpret_cast<v8h*>(at + 64 + 2 * o) = l;
+    }
 }
-__device__ __forceinline__ void put_operand(uint8_t* at, float x) {
-    const _Float16 h = static_cast<_Float16>(x);
-    *reinterpret_cast<_Float16*>(at) = h;
-    *reinterpret_cast<_Float16*>(at + 64) = static_cast<_Float16>(x - static_cast<float>(h));
+__device__ __forceinline__ void get_operand(const uint8_t* at, float (&x)[16]) {
+#pragma unroll
+    for (int o = 0; o < 16; o += 8) {
+        const v8h h = *reinterpret_cast<const v8h*>(at + 2 * o), l = *reinterpret_cast<const v8h*>(at + 64 + 2 * o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[o + e] = static_cast<float>(h[e]) + static_cast<float>(l[e]);
+    }
 }
 
 struct NsStart {
@@ -103,7 +135,7 @@ struct NsStart {
     uint8_t *x, *xt;
     NsFactors* factors;
     int rows, cols;           // of G as it lies
-    int tall, steps, parts;
+    int tall, steps, parts, vec;
     int64_t x_stride, xt_stride, x_matrix, xt_matrix;      // X has min(rows, cols) rows
     float eps;
     NsCoefficients k;
@@ -115,9 +147,14 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsStart p) {
     __shared__ float lds[64][65];
     const int64_t z = blockIdx.z;
     const int tid = threadIdx.x;
+    __shared__ double lds_norm[4];
     double norm = 0.0;
-    for (int i = 0; i < p.parts; ++i) norm += p.partial[z * p.parts + i];
-    norm = sqrt(norm);
+    for (int i = tid; i < p.parts; i += 256) norm += p.partial[z * p.parts + i];
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) norm += __shfl_xor(norm, w);
+    if ((tid & 63) == 0) lds_norm[tid >> 6] = norm;
+    __syncthreads();
+    norm = sqrt((lds_norm[0] + lds_norm[1]) + (lds_norm[2] + lds_norm[3]));
     const double inverse = norm < 1e300 ? 1.0 / (norm + static_cast<double>(p.eps)) : __longlong_as_double(0x7ff8000000000000ll);
     const double first = norm * inverse;
     const int e0 = operand_exponent(first);
@@ -145,17 +182,32 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const NsStart p) {
     uint8_t* const same = p.tall ? p.xt + z * p.xt_matrix : p.x + z * p.x_matrix;
     uint8_t* const turned = p.tall ? p.x + z * p.x_matrix : p.xt + z * p.xt_matrix;
     const int64_t same_stride = p.tall ? p.xt_stride : p.x_stride, turned_stride = p.tall ? p.x_stride : p.xt_stride;
-    for (int i = tid; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        float x = 0.0f;
-        if (r0 + r < p.rows && c0 + c < p.cols) x = static_cast<float>(static_cast<double>(to_f32(g[static_cast<int64_t>(r0 + r) * p.cols + c0 + c])) * factor);
-        lds[r][c] = x;
-        if (r0 + r < p.rows && (c0 + c) < (p.cols + 31) / 32 * 32) put_operand(same + operand_at(r0 + r, same_stride, c0 + c), x);
+    {
+        const int r = tid >> 2, c = (tid & 3) * 16;     // sixteen elements each
+        float x[16] = {};
+        if (r0 + r < p.rows) {
+            const T* const from = g + static_cast<int64_t>(r0 + r) * p.cols + c0 + c;
+            if (p.vec && c0 + c + 16 <= p.cols) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) load_f32<T, 4>(from + e, *reinterpret_cast<float (*)[4]>(x + e));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = c0 + c + e < p.cols ? to_f32(from[e]) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = c0 + c + e < p.cols ? static_cast<float>(static_cast<double>(x[e]) * factor) : 0.0f;
+            if (c0 + c < (p.cols + 31) / 32 * 32) put_operand(same + operand_at(r0 + r, same_stride, c0 + c), x);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) lds[r][c + e] = x[e];
     }
     __syncthreads();
-    for (int i = tid; i < 64 * 64; i += 256) {
-        const int c = i >> 6, r = i & 63;
-        if (c0 + c < p.cols && r0 + r < (p.rows + 31) / 32 * 32) put_operand(turned + operand_at(c0 + c, turned_stride, r0 + r), lds[r][c]);
+    {
+        const int c = tid & 63, r = (tid >> 6) * 16;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = lds[r + e][c];
+        if (c0 + c < p.cols && r0 + r < (p.rows + 31) / 32 * 32) put_operand(turned + operand_at(c0 + c, turned_stride, r0 + r), x);
     }
 }
 
@@ -168,15 +220,11 @@ struct NsProduct {
     int64_t a_matrix, b_matrix, added_matrix, added_stride, out_matrix, out_stride, turned_matrix, turned_stride, final_matrix;
     const NsFactors* factors;
     int which;                // 3 step + product
-    int tiles_m, tiles_n, stages, symmetric, final_turned;
+    int tiles_m, tiles_n, stages, symmetric, final_turned, final_vec;
 };
 
-template <class T, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(WM * WN * 64) void ns_product_kernel(const NsProduct p) {
-    typedef TileLoop<StepF16x2, WM, WN, TM, TN> Loop;
-    const int64_t z = blockIdx.y;
+__device__ __forceinline__ void ns_tile_of(const NsProduct& p, int& tm, int& tn) {
     int t = xcd_contiguous_index(blockIdx.x, gridDim.x);
-    int tm, tn;
     if (p.symmetric) {
         // the t-th tile on or above the diagonal, by rows
         tm = 0;
@@ -186,39 +234,129 @@ __global__ __launch_bounds__(WM * WN * 64) void ns_product_kernel(const NsProduc
         tm = t % p.tiles_m;
         tn = t / p.tiles_m;
     }
+}
+
+constexpr int NS_PITCH = 33;                            // floats from row to row of a block in LDS: rows and columns both meet different banks
+
+// A block of 32 x 32 sums, in LDS, becomes what the launch writes: by rows (half a row per lane), with what is added, then by columns.
+template <class T>
+__device__ __forceinline__ void ns_finish_block(const NsProduct& p, float* lds, int64_t z, int m0, int n0, bool mirror, float of_sum, float of_added) {
+    const int lane = threadIdx.x & 63, line = lane >> 1, part = (lane & 1) * 16;
+    const int M = p.a.rows, N = p.b.rows;
+    T* const final = p.final ? static_cast<T*>(p.final) + z * p.final_matrix : nullptr;
+    const auto put_final = [&](T* to, const float (&x)[16], int left) {
+        if (p.final_vec && left >= 16) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) store_f32<T, 4>(to + e, *reinterpret_cast<const float (*)[4]>(x + e));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (e < left) to[e] = from_f32<T>(x[e]);
+        }
+    };
+    float x[16];
+    {
+        const int m = m0 + line, n = n0 + part;
+        float* const row = lds + line * NS_PITCH + part;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = row[e] * of_sum;
+        if (p.added && m < M && n0 < N) {
+            float y[16];
+            get_operand(p.added + z * p.added_matrix + operand_at(m, p.added_stride, n), y);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = fmaf(y[e], of_added, x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if (m >= M || n + e >= N) x[e] = 0.0f;
+            row[e] = x[e];
+        }
+        if (m < M && n0 < N) {
+            if (!final) put_operand(p.out + z * p.out_matrix + operand_at(m, p.out_stride, n), x);
+            else if (!p.final_turned) put_final(final + static_cast<int64_t>(m) * N + n, x, N - n);
+        }
+    }
+    uint8_t* const turned = final ? nullptr : mirror ? p.out + z * p.out_matrix : p.turned ? p.turned + z * p.turned_matrix : nullptr;
+    if (!turned && !(final && p.final_turned)) return;
+    wave_fence();
+    {
+        const int n = n0 + line, m = m0 + part;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = lds[(part + e) * NS_PITCH + line];
+        if (n < N && m0 < M) {
+            if (turned) put_operand(turned + operand_at(n, mirror ? p.out_stride : p.turned_stride, m), x);
+            else put_final(final + static_cast<int64_t>(n) * M + m, x, M - m);
+        }
+    }
+}
+
+template <class T, class Loop>
+__global__ __launch_bounds__(Loop::THREADS, 2) void ns_product_kernel(const NsProduct p) {
+    constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN;
+    __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
+    const int64_t z = blockIdx.y;
+    int tm, tn;
+    ns_tile_of(p, tm, tn);
     const int m0 = tm * Loop::BM, n0 = tn * Loop::BN;
     RowBytes A = p.a, B = p.b;
     A.base += z * p.a_matrix;
     B.base += z * p.b_matrix;
     v4f acc[TM][TN];
-    Loop::run(A, B, m0, n0, p.stages, acc);
+    Loop::run(A, B, m0, n0, p.stages, even, odd, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int mw = m0 + wave / WN * TM * 16 + (lane >> 4) * 4, nw = n0 + wave % WN * TN * 16 + (lane & 15);
     const float of_sum = p.factors[z].of_sum[p.which], of_added = p.factors[z].of_added[p.which];
-    const int M = A.rows, N = B.rows, M32 = (M + 31) / 32 * 32, N32 = (N + 31) / 32 * 32;
+    static_assert(Loop::WAVES * 32 * NS_PITCH * 4 <= Loop::STAGE, "a block per wave fits a stage");
+    __syncthreads();                                    // every wave has read its last stage
+    float* const lds = reinterpret_cast<float*>(even) + wave * 32 * NS_PITCH;
     const bool mirror = p.symmetric && tm != tn;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; i += 2)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+        for (int j = 0; j < TN; j += 2) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int m = mw + 16 * i + r, n = nw + 16 * j;
-                const bool inside = m < M && n < N;
-                float v = 0.0f;
-                if (inside) {
-                    v = acc[i][j][r] * of_sum;
-                    if (p.added) v = fmaf(operand_value(p.added + z * p.added_matrix + operand_at(m, p.added_stride, n)), of_added, v);
-                }
-                if (p.final) {
-                    T* const y = static_cast<T*>(p.final) + z * p.final_matrix;
-                    if (inside) y[p.final_turned ? static_cast<int64_t>(n) * M + m : static_cast<int64_t>(m) * N + n] = from_f32<T>(v);
-                } else {
-                    if (m < M && n < N32) put_operand(p.out + z * p.out_matrix + operand_at(m, p.out_stride, n), v);
-                    if (mirror && n < N && m < M32) put_operand(p.out + z * p.out_matrix + operand_at(n, p.out_stride, m), v);
-                    if (p.turned && n < N && m < M32) put_operand(p.turned + z * p.turned_matrix + operand_at(n, p.turned_stride, m), v);
-                }
-            }
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) lds[(16 * u + (lane >> 4) * 4 + r) * NS_PITCH + 16 * v + (lane & 15)] = acc[i + u][j + v][r];
+            wave_fence();
+            ns_finish_block<T>(p, lds, z, m0 + (wave / WN * TM + i) * 16, n0 + (wave % WN * TN + j) * 16, mirror, of_sum, of_added);
+            wave_fence();
+        }
+}
+
+// A tile of 32 x 32 per work-group, its waves each a share of K
+template <class T, int WAVES, int DEEP>
+__global__ __launch_bounds__(WAVES * 64) void ns_small_kernel(const NsProduct p) {
+    typedef TileSplit<StepF16x2, WAVES, 2, 2, DEEP> Split;
+    __shared__ float lds[WAVES][32 * NS_PITCH];
+    const int64_t z = blockIdx.y;
+    int tm, tn;
+    ns_tile_of(p, tm, tn);
+    const int m0 = tm * Split::BM, n0 = tn * Split::BN;
+    RowBytes A = p.a, B = p.b;
+    A.base += z * p.a_matrix;
+    B.base += z * p.b_matrix;
+    v4f acc[2][2];
+    Split::run(A, B, m0, n0, p.stages, acc);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float of_sum = p.factors[z].of_sum[p.which], of_added = p.factors[z].of_added[p.which];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds[wave][(16 * u + (lane >> 4) * 4 + r) * NS_PITCH + 16 * v + (lane & 15)] = acc[u][v][r];
+    __syncthreads();
+    for (int i = tid; i < 32 * 32; i += WAVES * 64) {
+        const int at = (i >> 5) * NS_PITCH + (i & 31);
+        float sum = lds[0][at];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum += lds[w][at];
+        lds[0][at] = sum;
+    }
+    __syncthreads();
+    if (wave == 0) ns_finish_block<T>(p, lds[0], z, m0, n0, p.symmetric && tm != tn, of_sum, of_added);
 }
 
 // ------------------------------------------------------------------------------------------------------------ host side
@@ -249,6 +387,13 @@ NsLayout ns_layout(int64_t batch, int64_t rows, int64_t cols) {
     return l;
 }
 
+// Work-groups that add up a matrix: 4096 elements each as long as all together stay below four per CU
+int ns_norm_blocks(int64_t batch, int64_t count) {
+    const int64_t wanted = (count + 4095) / 4096, most = 4 * device_cu_count() / batch;
+    const int64_t n = wanted < most ? wanted : most;
+    return static_cast<int>(n < 1 ? 1 : (n < NS_NORM_BLOCKS ? n : NS_NORM_BLOCKS));
+}
+
 bool ns_fits(int64_t batch, int64_t rows, int64_t cols) {
     return batch > 0 && batch <= 65535 && rows > 0 && cols > 0 && rows <= NS_MOST_SIDE && cols <= NS_MOST_SIDE;
 }
@@ -260,12 +405,13 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
     double* const partial = reinterpret_cast<double*>(ws + l.partial);
     NsFactors* const factors = reinterpret_cast<NsFactors*>(ws + l.factors);
     const int64_t count = rows * cols;
-    int norm_blocks = static_cast<int>((count + 4095) / 4096 < NS_NORM_BLOCKS ? (count + 4095) / 4096 : NS_NORM_BLOCKS);
-    hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(norm_blocks, static_cast<unsigned>(batch)), dim3(256), 0, stream, static_cast<const T*>(g), count, partial);
+    const int norm_blocks = ns_norm_blocks(batch, count);
+    const int vec = cols % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0, out_vec = cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(norm_blocks, static_cast<unsigned>(batch)), dim3(256), 0, stream, static_cast<const T*>(g), count, partial, vec);
     NsStart s{};
     s.g = g; s.partial = partial; s.x = ws + l.x; s.xt = ws + l.xt; s.factors = factors;
     s.rows = static_cast<int>(rows); s.cols = static_cast<int>(cols);
-    s.tall = rows > cols; s.steps = steps; s.parts = norm_blocks;
+    s.tall = rows > cols; s.steps = steps; s.parts = norm_blocks; s.vec = vec;
     s.x_stride = l.x_stride; s.xt_stride = l.xt_stride; s.x_matrix = l.m * l.x_stride; s.xt_matrix = l.n * l.xt_stride;
     s.eps = eps; s.k = k;
     hipLaunchKernelGGL((ns_start_kernel<T>), dim3(static_cast<unsigned>((cols + 63) / 64), static_cast<unsigned>((rows + 63) / 64), static_cast<unsigned>(batch)), dim3(256),
@@ -274,10 +420,24 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
     const int64_t sq_matrix = l.m * l.sq_stride;
     const auto product = [&](NsProduct p) {
         p.factors = factors;
-        p.tiles_m = (p.a.rows + 127) / 128;
-        p.tiles_n = (p.b.rows + 127) / 128;
-        const int64_t tiles = p.symmetric ? static_cast<int64_t>(p.tiles_n) * (p.tiles_n + 1) / 2 : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-        hipLaunchKernelGGL((ns_product_kernel<T, 2, 2, 4, 4>), dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(batch)), dim3(256), 0, stream, p);
+        p.final_vec = out_vec;
+        const auto tiles = [&](int side) {
+            p.tiles_m = (p.a.rows + side - 1) / side;
+            p.tiles_n = (p.b.rows + side - 1) / side;
+            return p.symmetric ? static_cast<int64_t>(p.tiles_n) * (p.tiles_n + 1) / 2 : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+        };
+        if (tiles(128) * batch < device_cu_count()) {
+            const dim3 grid(static_cast<unsigned>(tiles(32)), static_cast<unsigned>(batch));
+            if (p.stages > 4) hipLaunchKernelGGL((ns_small_kernel<T, 8, 3>), grid, dim3(512), 0, stream, p);
+            else              hipLaunchKernelGGL((ns_small_kernel<T, 4, 1>), grid, dim3(256), 0, stream, p);
+        } else {
+            typedef TileLoop<StepF16x2, 2, 2, 4, 4> Loop;
+            typedef TilePingPong<StepF16x2> Large;
+            if (tiles(256) * batch >= device_cu_count())
+                hipLaunchKernelGGL((ns_product_kernel<T, Large>), dim3(static_cast<unsigned>(tiles(256)), static_cast<unsigned>(batch)), dim3(Large::THREADS), 0, stream, p);
+            else
+                hipLaunchKernelGGL((ns_product_kernel<T, Loop>), dim3(static_cast<unsigned>(tiles(128)), static_cast<unsigned>(batch)), dim3(Loop::THREADS), 0, stream, p);
+        }
     };
     const int m = static_cast<int>(l.m), n = static_cast<int>(l.n);
     for (int step = 0; step < steps; ++step) {

@@ -31,7 +31,7 @@ def test_product(lib):
     need = lib.mul_mat_i8_workspace_hip(3, 40)
     assert need >= 3 * 128 + 12 and lib.mul_mat_i8_workspace_hip(0, 40) == 0 and lib.mul_mat_i8_workspace_hip(3, 131072) == 0
     ok = dict(w=ONE, ws=ONE, x=ONE, xt=0, stride=40, xs=None, bias=None, y=ONE, yt=0, M=5, N=3, K=40, wsp=ONE, nbytes=need)
-    for bad in (dict(w=None), dict(ws=None), dict(x=None), dict(y=None), dict(M=0), dict(N=0), dict(K=0), dict(K=131072, stride=131072), dict(stride=39), dict(yt=3),
+    for bad in (dict(w=None), dict(ws=None), dict(x=None), dict(y=None), dict(M=0), dict(M=(1 << 22) + 1), dict(N=0), dict(K=0), dict(K=131072, stride=131072), dict(stride=39), dict(yt=3),
                 dict(yt=9), dict(xt=5), dict(xt=3), dict(w=C.c_void_p(4097)), dict(wsp=None), dict(nbytes=need - 1), dict(wsp=C.c_void_p(4100))):
         a = dict(ok, **bad)
         assert lib.mul_mat_i8_hip(a["w"], a["ws"], a["x"], a["xt"], a["stride"], a["xs"], a["bias"], a["y"], a["yt"], a["M"], a["N"], a["K"], a["wsp"], a["nbytes"], None) == 1, bad

@@ -54,8 +54,8 @@ def weight(gen, m, k):
 
 
 # one token to several tiles; k below, at and above a stage of 128 bytes; channels below a tile and ragged
-SHAPES = [(1, 1, 1), (1, 32, 1), (2, 127, 3), (3, 128, 130), (1, 4096, 4096), (1, 500, 1001), (7, 129, 64), (8, 1024, 257), (15, 256, 768), (16, 250, 96),
-          (17, 384, 33), (33, 96, 256), (65, 640, 200), (130, 257, 129), (408, 256, 256), (300, 1100, 300), (513, 2048, 513), (1030, 72, 24)]
+SHAPES = [(1, 1, 1), (1, 32, 1), (5, 3, 7), (70, 2, 130), (40, 4, 20), (40, 5, 64), (300, 6, 64), (300, 7, 65), (2, 127, 3), (3, 128, 130), (1, 4096, 4096), (1, 500, 1001), (7, 129, 64), (8, 1024, 257), (15, 256, 768), (16, 250, 96),
+          (17, 384, 33), (3, 5300, 40), (4, 4096, 48), (5, 2048, 20), (2, 8190, 16), (1, 16380, 24), (1, 16400, 24), (13, 1999, 33), (33, 96, 256), (500, 380, 513), (900, 512, 1030), (65, 640, 200), (130, 257, 129), (408, 256, 256), (300, 1100, 300), (513, 2048, 513), (1030, 72, 24)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -75,6 +75,20 @@ def test_linear_matches_the_definition(ops, n, k, m, dtype):
     # the same bits from a weight that is laid out in the call, and from activations quantized ahead
     assert torch.equal(ops.mul_mat_i8(W, x, bias), got)
     assert torch.equal(ops.mul_mat_i8(W.pack(), (q, scale), bias, dtype=dtype), got)
+
+
+# one to several stages of 128 bytes under enough tiles for the largest form, ragged on either side
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [(4100, 100, 4100), (4097, 130, 4352), (3900, 300, 4300), (8200, 512, 2060)])
+def test_large_linear(ops, n, k, m, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(n, k, device="cuda", generator=gen).to(dtype)
+    w, ws = weight(gen, m, k)
+    bias = torch.randn(m, device="cuda", generator=gen)
+    q, scale = rule(x)
+    got = ops.mul_mat_i8(ops.I8Weight(w, ws), x, bias)
+    check(got, q, scale, w, ws, bias)
+    assert torch.equal(ops.mul_mat_i8(ops.I8Weight(w, ws), x[17:300], bias), got[17:300])
 
 
 @pytest.mark.parametrize("out", TYPES)

@@ -66,6 +66,14 @@ def test_matches_the_iteration(ops, shape, steps):
     check(ops.newton_schulz(g, steps=steps), g, steps)
 
 
+# stacks large enough for the forms with tiles of 128 and 256
+@pytest.mark.parametrize("shape", [(90, 260, 300), (90, 400, 257), (40, 270, 300), (300, 96, 130)])
+def test_large_stacks(ops, shape):
+    g = update(shape, seed=11)
+    for steps in (1, 2):
+        check(ops.newton_schulz(g, steps=steps), g, steps)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(24, 72), (3, 100, 64), (160, 160)])
 def test_types(ops, shape, dtype):
