@@ -77,9 +77,13 @@ __device__ __forceinline__ float group_sum(float v, int group) {
 }
 
 // What a lane holds of a head: R chunks of two times V elements.  A chunk's halves `a`, `b` are V pairs' first and second
-// elements (half-split) or 2 V consecutive elements (interleaved, and behind the rotated ones).
-template <int V, int R>
+// elements (half-split) or 2 V consecutive elements (interleaved, and behind the rotated ones).  FULL: a head is as many chunks as the group
+// has lanes, so that none is outside, and no load or store stands under a condition (the compiler then waits for a head's loads alone, not
+// for the stores behind them).
+template <class T, int V, int R, bool FULL>
 struct Chunks {
+    typedef typename Elements<T, V>::Raw Raw;
+    struct Head { Raw a[R], b[R]; };
     int at_a[R], at_b[R];     // -1: outside the head
     float sine[R][V], cosine[R][V];
 
@@ -124,22 +128,42 @@ struct Chunks {
                 x = t;
             }
     }
-    template <class T>
-    __device__ __forceinline__ void load(const T* head, float (&a)[R][V], float (&b)[R][V], float fill = 0.0f) const {
+    __device__ __forceinline__ Head fetch(const T* head) const {
+        Head x;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) a[r][v] = b[r][v] = fill;
-            if (at_a[r] >= 0) load_f32<T, V>(head + at_a[r], a[r]);
-            if (at_b[r] >= 0) load_f32<T, V>(head + at_b[r], b[r]);
+            x.a[r] = *reinterpret_cast<const Raw*>(head + (FULL || at_a[r] >= 0 ? at_a[r] : 0));
+            x.b[r] = *reinterpret_cast<const Raw*>(head + (FULL || at_b[r] >= 0 ? at_b[r] : 0));
         }
+        return x;
     }
-    template <class T>
-    __device__ __forceinline__ void store(T* head, const float (&a)[R][V], const float (&b)[R][V]) const {
+    __device__ __forceinline__ void finish(const Head& x, float (&a)[R][V], float (&b)[R][V]) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if constexpr (V == 1) { a[r][v] = to_f32(static_cast<T>(x.a[r])); b[r][v] = to_f32(static_cast<T>(x.b[r])); }
+                else                  { a[r][v] = to_f32(static_cast<T>(x.a[r][v])); b[r][v] = to_f32(static_cast<T>(x.b[r][v])); }
+                if (!FULL && at_a[r] < 0) a[r][v] = 0.0f;
+                if (!FULL && at_b[r] < 0) b[r][v] = 0.0f;
+            }
+    }
+    // of the norms' weights (a lane's own few, once)
+    __device__ __forceinline__ void load_weights(const float* w, float (&a)[R][V], float (&b)[R][V]) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                a[r][v] = at_a[r] >= 0 ? w[at_a[r] + v] : 0.0f;
+                b[r][v] = at_b[r] >= 0 ? w[at_b[r] + v] : 0.0f;
+            }
+    }
+    template <class U>
+    __device__ __forceinline__ void store(U* head, const float (&a)[R][V], const float (&b)[R][V]) const {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (at_a[r] >= 0) store_f32<T, V>(head + at_a[r], a[r]);
-            if (at_b[r] >= 0) store_f32<T, V>(head + at_b[r], b[r]);
+            if (FULL || at_a[r] >= 0) store_f32<U, V>(head + at_a[r], a[r]);
+            if (FULL || at_b[r] >= 0) store_f32<U, V>(head + at_b[r], b[r]);
         }
     }
 };
@@ -151,44 +175,58 @@ __device__ __forceinline__ double position_of(const HeadNorm& p, int64_t b, int6
                            : static_cast<double>(static_cast<const int64_t*>(p.positions)[at]);
 }
 
-template <class T, int V, int R, bool INTER>
+// What both passes have of a head's elements
+template <int R, int V>
+__device__ __forceinline__ float squares_of(const float (&a)[R][V], const float (&b)[R][V]) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum = fmaf(a[r][v], a[r][v], fmaf(b[r][v], b[r][v], sum));
+    return sum;
+}
+
+template <class T, int V, int R, bool INTER, bool FULL>
 __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNorm p) {
     const int lane = threadIdx.x & (p.group - 1);
     const int64_t token = static_cast<int64_t>(blockIdx.x) * (256 / p.group) + threadIdx.x / p.group;
     if (token >= p.tokens) return;                      // (whole groups)
     const int64_t b = token / p.L, l = token % p.L;
-    Chunks<V, R> ch;
+    Chunks<T, V, R, FULL> ch;
     ch.place(lane, p.group, p.d, p.rot, INTER);
-    ch.angles(lane, p.group, p, position_of(p, b, l));
     const int all = p.side[0].heads + p.side[1].heads;
     const int first = blockIdx.y * p.heads_per_part, end = first + p.heads_per_part < all ? first + p.heads_per_part : all;
     const float mean = 1.0f / static_cast<float>(p.d);
+    bool turned = false;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const HeadSide& side = p.side[s];
         const int before = s == 0 ? 0 : p.side[0].heads;
-        int h = first - before > 0 ? first - before : 0;
-        const int stop = end - before < side.heads ? end - before : side.heads;
-        if (h >= stop) continue;
-        float wa[R][V], wb[R][V];
-        if (side.w) ch.load(side.w, wa, wb);
+        const int begin = first - before > 0 ? first - before : 0, stop = end - before < side.heads ? end - before : side.heads;
+        if (begin >= stop) continue;
         const T* const x = static_cast<const T*>(side.x) + b * side.x_b + l * side.x_l;
         T* const y = static_cast<T*>(side.out) + b * side.out_b + l * side.out_l;
-        for (; h < stop; ++h) {
-            float xa[R][V], xb[R][V];
-            ch.load(x + h * side.x_h, xa, xb);
-            float squares = 0.0f;
+        typename Chunks<T, V, R, FULL>::Head next = ch.fetch(x + begin * side.x_h);
+        if (!turned) ch.angles(lane, p.group, p, position_of(p, b, l));
+        turned = true;
+        float wa[R][V], wb[R][V];
+        if (side.w) ch.load_weights(side.w, wa, wb);
+        else
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int v = 0; v < V; ++v) squares = fmaf(xa[r][v], xa[r][v], fmaf(xb[r][v], xb[r][v], squares));
-            const float scale = rsqrtf(fmaf(group_sum(squares, p.group), mean, p.eps));
+                for (int v = 0; v < V; ++v) wa[r][v] = wb[r][v] = 1.0f;
+        for (int h = begin; h < stop; ++h) {
+            float xa[R][V], xb[R][V];
+            ch.finish(next, xa, xb);
+            next = ch.fetch(x + (h + 1 < stop ? h + 1 : h) * side.x_h);      // (past the last head, that one again)
+            const float scale = rsqrtf(fmaf(group_sum(squares_of(xa, xb), p.group), mean, p.eps));
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    xa[r][v] *= side.w ? scale * wa[r][v] : scale;
-                    xb[r][v] *= side.w ? scale * wb[r][v] : scale;
+                    xa[r][v] *= scale * wa[r][v];
+                    xb[r][v] *= scale * wb[r][v];
                 }
             ch.template rotate<INTER, false>(xa, xb);
             ch.store(y + h * side.out_h, xa, xb);
@@ -196,41 +234,49 @@ __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNorm p) {
     }
 }
 
-template <class T, int V, int R, bool INTER>
+template <class T, int V, int R, bool INTER, bool FULL>
 __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
     extern __shared__ __attribute__((aligned(16))) float lds[];      // [tokens of the work-group][d]
     const int lane = threadIdx.x & (p.group - 1), groups = 256 / p.group, mine = threadIdx.x / p.group;
-    Chunks<V, R> ch;
+    Chunks<T, V, R, FULL> ch;
+    typedef typename Chunks<T, V, R, FULL>::Head Head;
     ch.place(lane, p.group, p.d, p.rot, INTER);
     const int all = p.side[0].heads + p.side[1].heads;
     const int first = blockIdx.y * p.heads_per_part, end = first + p.heads_per_part < all ? first + p.heads_per_part : all;
     const float mean = 1.0f / static_cast<float>(p.d);
-    float dwa[2][R][V] = {}, dwb[2][R][V] = {};
+    float wa[2][R][V], wb[2][R][V], dwa[2][R][V] = {}, dwb[2][R][V] = {};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if (p.side[s].w) ch.load_weights(p.side[s].w, wa[s], wb[s]);
+        else
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int v = 0; v < V; ++v) wa[s][r][v] = wb[s][r][v] = 1.0f;
+    }
     for (int64_t token = static_cast<int64_t>(blockIdx.x) * groups + mine; token < p.tokens; token += static_cast<int64_t>(gridDim.x) * groups) {
         const int64_t b = token / p.L, l = token % p.L;
-        ch.angles(lane, p.group, p, position_of(p, b, l));
+        bool turned = false;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const HeadSide& side = p.side[s];
             const int before = s == 0 ? 0 : p.side[0].heads;
-            int h = first - before > 0 ? first - before : 0;
-            const int stop = end - before < side.heads ? end - before : side.heads;
-            if (h >= stop) continue;
-            float wa[R][V], wb[R][V];
-            if (side.w) ch.load(side.w, wa, wb);
+            const int begin = first - before > 0 ? first - before : 0, stop = end - before < side.heads ? end - before : side.heads;
+            if (begin >= stop) continue;
             const T* const x = static_cast<const T*>(side.x) + b * side.x_b + l * side.x_l;
             const T* const dy = static_cast<const T*>(side.dy) + b * side.dy_b + l * side.dy_l;
             T* const dx = static_cast<T*>(side.out) + b * side.out_b + l * side.out_l;
-            for (; h < stop; ++h) {
+            Head next_x = ch.fetch(x + begin * side.x_h), next_g = ch.fetch(dy + begin * side.dy_h);
+            if (!turned) ch.angles(lane, p.group, p, position_of(p, b, l));
+            turned = true;
+            for (int h = begin; h < stop; ++h) {
                 float xa[R][V], xb[R][V], ga[R][V], gb[R][V];
-                ch.load(x + h * side.x_h, xa, xb);
-                ch.load(dy + h * side.dy_h, ga, gb);
-                float squares = 0.0f;
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) squares = fmaf(xa[r][v], xa[r][v], fmaf(xb[r][v], xb[r][v], squares));
-                const float scale = rsqrtf(fmaf(group_sum(squares, p.group), mean, p.eps));
+                ch.finish(next_x, xa, xb);
+                ch.finish(next_g, ga, gb);
+                const int after = h + 1 < stop ? h + 1 : h;
+                next_x = ch.fetch(x + after * side.x_h);
+                next_g = ch.fetch(dy + after * side.dy_h);
+                const float scale = rsqrtf(fmaf(group_sum(squares_of(xa, xb), p.group), mean, p.eps));
                 ch.template rotate<INTER, true>(ga, gb);
                 float along = 0.0f;
 #pragma unroll
@@ -239,12 +285,10 @@ __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
                     for (int v = 0; v < V; ++v) {
                         xa[r][v] *= scale;
                         xb[r][v] *= scale;
-                        if (side.w) {
-                            dwa[s][r][v] = fmaf(ga[r][v], xa[r][v], dwa[s][r][v]);
-                            dwb[s][r][v] = fmaf(gb[r][v], xb[r][v], dwb[s][r][v]);
-                            ga[r][v] *= wa[r][v];
-                            gb[r][v] *= wb[r][v];
-                        }
+                        dwa[s][r][v] = fmaf(ga[r][v], xa[r][v], dwa[s][r][v]);
+                        dwb[s][r][v] = fmaf(gb[r][v], xb[r][v], dwb[s][r][v]);
+                        ga[r][v] *= wa[s][r][v];
+                        gb[r][v] *= wb[s][r][v];
                         along = fmaf(ga[r][v], xa[r][v], fmaf(gb[r][v], xb[r][v], along));
                     }
                 along = group_sum(along, p.group) * mean;
@@ -265,7 +309,7 @@ __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
     for (int s = 0; s < 2; ++s) {
         if (!p.side[s].w) continue;
         __syncthreads();
-        ch.store(lds + mine * p.d, dwa[s], dwb[s]);
+        ch.template store<float>(lds + mine * p.d, dwa[s], dwb[s]);
         __syncthreads();
         for (int e = threadIdx.x; e < p.d; e += 256) {
             float sum = 0.0f;
@@ -275,20 +319,28 @@ __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
     }
 }
 
-// dw[e] = the sum over `parts` work-groups of partial[part][side][e]: 16 threads per element, each a run of parts in their order
+// dw[e] = the sum over `parts` work-groups of partial[part][side][e].  A work-group takes eight elements, 32 threads each: a thread every 32nd part,
+// eight of them on their way at once (a chain of loads 21 us for 1024 parts of 32 elements).
 __global__ __launch_bounds__(256) void head_norm_weights_kernel(const float* partial, int parts, int d, float* dwq, float* dwk) {
-    __shared__ float lds[16][17];
-    const int col = threadIdx.x & 15, run = threadIdx.x >> 4;
-    const int e = blockIdx.x * 16 + col, s = blockIdx.y;
+    __shared__ float lds[32][9];
+    const int col = threadIdx.x & 7, run = threadIdx.x >> 3;
+    const int e = blockIdx.x * 8 + col, s = blockIdx.y;
     float* const dw = s == 0 ? dwq : dwk;
     if (!dw) return;
+    const float* const from = partial + s * d + (e < d ? e : d - 1);
+    const int64_t step = 2 * static_cast<int64_t>(d);
     float sum = 0.0f;
-    if (e < d)
-        for (int i = run; i < parts; i += 16) sum += partial[(static_cast<int64_t>(i) * 2 + s) * d + e];
+    for (int i = run; i < parts; i += 32 * 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = from[(i + 32 * u < parts ? i + 32 * u : run) * step];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum += i + 32 * u < parts ? x[u] : 0.0f;
+    }
     lds[run][col] = sum;
     __syncthreads();
     if (run == 0 && e < d) {
-        for (int i = 1; i < 16; ++i) sum += lds[i][col];
+        for (int i = 1; i < 32; ++i) sum += lds[i][col];
         dw[e] = sum;
     }
 }
@@ -296,20 +348,26 @@ __global__ __launch_bounds__(256) void head_norm_weights_kernel(const float* par
 constexpr int HEAD_MAX_D = 512;
 constexpr int BACK_MOST_BLOCKS = 1024;
 
-struct HeadPlan { bool vec; int chunks, group, chunks_per_lane; unsigned blocks, parts; };
+struct HeadPlan { int v, chunks_per_lane, group; bool full; unsigned blocks, parts; };
 
-size_t elem_bytes(int type) { return type == PPML_ELEM_F32 ? 4 : 2; }
+int elem_bytes(int type) { return type == PPML_ELEM_F32 ? 4 : 2; }
 
-// how a head is dealt to lanes: the layout allows four elements at a time, or one
-HeadPlan plan_heads(const ppml_qk_norm_desc& a, bool aligned, bool back) {
+// How a head is dealt to lanes.  `aligned`: to how many elements at a time (1, 4, 8) addresses and strides are multiples of; sixteen bytes are
+// taken where the head's parts are whole pieces of as many.
+HeadPlan plan_heads(const ppml_qk_norm_desc& a, int aligned, bool back) {
     HeadPlan pl{};
-    const bool whole = a.interleaved ? a.d % 8 == 0 && a.rot % 8 == 0 : a.rot % 8 == 0 && (a.d - a.rot) % 8 == 0;
-    pl.vec = aligned && whole;
-    pl.chunks = pl.vec ? a.d / 8 : (a.d + 1) / 2;
+    const auto whole = [&](int v) { return aligned % v == 0 && (a.interleaved ? a.d % (2 * v) == 0 && a.rot % (2 * v) == 0 : a.rot % (2 * v) == 0 && (a.d - a.rot) % (2 * v) == 0); };
+    // Eight elements at a time halve the instructions per head and double the angles per lane: for tokens enough to fill the chip with half of the
+    // lanes (bf16, 32768 tokens of 40 heads of 128 141 us, 182 with four; 16384 of 32 heads of 64 25.4 / 27.0; 26368 of 16 heads of 32 15.2 / 13.6; one token
+    // 4.2 / 3.5)
+    const int64_t tokens = a.B * a.L;
+    pl.v = a.type != PPML_ELEM_F32 && whole(8) && tokens * (a.d / 16) >= 65536 ? 8 : whole(4) ? 4 : 1;
+    const int chunks = (a.d + 2 * pl.v - 1) / (2 * pl.v);
     pl.group = 1;
-    while (pl.group < 64 && pl.group < pl.chunks) pl.group *= 2;
-    pl.chunks_per_lane = (pl.chunks + pl.group - 1) / pl.group;
-    const int64_t tokens = a.B * a.L, per_block = 256 / pl.group;
+    while (pl.group < 64 && pl.group < chunks) pl.group *= 2;
+    pl.full = chunks == pl.group && a.d % (2 * pl.v) == 0;
+    pl.chunks_per_lane = (chunks + pl.group - 1) / pl.group;
+    const int64_t per_block = 256 / pl.group;
     int64_t blocks = (tokens + per_block - 1) / per_block;
     const int heads = a.hq + a.hk;
     if (back && blocks > BACK_MOST_BLOCKS) blocks = BACK_MOST_BLOCKS;
@@ -327,34 +385,42 @@ bool desc_ok(const ppml_qk_norm_desc* a) {
            (a->position_bytes == 0 || a->position_bytes == 4 || a->position_bytes == 8) && a->B * a->L <= (int64_t{1} << 32);
 }
 
-bool side_aligned(const HeadSide& s, size_t elem, bool back) {
-    if (s.heads == 0) return true;
-    const uintptr_t bytes = 4 * elem;
-    const auto ok = [&](const void* ptr, int64_t b, int64_t l, int64_t h) {
-        return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && b % 4 == 0 && l % 4 == 0 && h % 4 == 0;
-    };
-    return ok(s.x, s.x_b, s.x_l, s.x_h) && ok(s.out, s.out_b, s.out_l, s.out_h) && (!back || ok(s.dy, s.dy_b, s.dy_l, s.dy_h)) &&
-           reinterpret_cast<uintptr_t>(s.w) % 16 == 0;
+// elements that all of a side's addresses and steps are multiples of: 8, 4 or 1
+int side_aligned(const HeadSide& s, int elem, bool back) {
+    if (s.heads == 0) return 8;
+    for (const int v : {8, 4}) {
+        const auto ok = [&](const void* ptr, int64_t b, int64_t l, int64_t h) {
+            return reinterpret_cast<uintptr_t>(ptr) % static_cast<uintptr_t>(v * elem) == 0 && b % v == 0 && l % v == 0 && h % v == 0;
+        };
+        if (ok(s.x, s.x_b, s.x_l, s.x_h) && ok(s.out, s.out_b, s.out_l, s.out_h) && (!back || ok(s.dy, s.dy_b, s.dy_l, s.dy_h))) return v;
+    }
+    return 1;
+}
+int both_aligned(const HeadNorm& p, int elem, bool back) {
+    const int q = side_aligned(p.side[0], elem, back), k = side_aligned(p.side[1], elem, back);
+    return q < k ? q : k;
 }
 
-template <class T, int V, int R>
+template <class T, int V, int R, bool FULL>
 void launch_heads(const HeadNorm& p, const HeadPlan& pl, bool back, hipStream_t stream) {
     const dim3 grid(pl.blocks, pl.parts), block(256);
     const size_t lds = back ? static_cast<size_t>(256 / p.group) * p.d * 4 : 0;
     if (back) {
-        if (p.interleaved) hipLaunchKernelGGL((head_norm_back_kernel<T, V, R, true>), grid, block, lds, stream, p);
-        else               hipLaunchKernelGGL((head_norm_back_kernel<T, V, R, false>), grid, block, lds, stream, p);
+        if (p.interleaved) hipLaunchKernelGGL((head_norm_back_kernel<T, V, R, true, FULL>), grid, block, lds, stream, p);
+        else               hipLaunchKernelGGL((head_norm_back_kernel<T, V, R, false, FULL>), grid, block, lds, stream, p);
     } else {
-        if (p.interleaved) hipLaunchKernelGGL((head_norm_kernel<T, V, R, true>), grid, block, 0, stream, p);
-        else               hipLaunchKernelGGL((head_norm_kernel<T, V, R, false>), grid, block, 0, stream, p);
+        if (p.interleaved) hipLaunchKernelGGL((head_norm_kernel<T, V, R, true, FULL>), grid, block, 0, stream, p);
+        else               hipLaunchKernelGGL((head_norm_kernel<T, V, R, false, FULL>), grid, block, 0, stream, p);
     }
 }
 
 template <class T>
 void launch_heads(const HeadNorm& p, const HeadPlan& pl, bool back, hipStream_t stream) {
-    if (pl.vec) launch_heads<T, 4, 1>(p, pl, back, stream);
-    else if (pl.chunks_per_lane == 1) launch_heads<T, 1, 1>(p, pl, back, stream);
-    else launch_heads<T, 1, 4>(p, pl, back, stream);
+    if constexpr (sizeof(T) == 2)
+        if (pl.v == 8) return pl.full ? launch_heads<T, 8, 1, true>(p, pl, back, stream) : launch_heads<T, 8, 1, false>(p, pl, back, stream);
+    if (pl.v == 4) return pl.full ? launch_heads<T, 4, 1, true>(p, pl, back, stream) : launch_heads<T, 4, 1, false>(p, pl, back, stream);
+    if (pl.chunks_per_lane == 1) return launch_heads<T, 1, 1, false>(p, pl, back, stream);
+    launch_heads<T, 1, 4, false>(p, pl, back, stream);
 }
 
 int run_heads(const ppml_qk_norm_desc& a, HeadNorm p, const HeadPlan& pl, bool back, hipStream_t stream, const char* what) {
@@ -406,16 +472,15 @@ extern "C" int qk_norm_rope_hip(const ppml_qk_norm_desc* a, const void* q, const
     HeadNorm p = describe(*a, freqs, positions);
     p.side[0] = side_of(q, a->q_strides, nullptr, nullptr, q_out, a->q_out_strides, wq, a->hq);
     p.side[1] = side_of(k, a->k_strides, nullptr, nullptr, k_out, a->k_out_strides, wk, a->hk);
-    const size_t elem = elem_bytes(a->type);
-    const HeadPlan pl = plan_heads(*a, side_aligned(p.side[0], elem, false) && side_aligned(p.side[1], elem, false), false);
+    const HeadPlan pl = plan_heads(*a, both_aligned(p, elem_bytes(a->type), false), false);
     return run_heads(*a, p, pl, false, static_cast<hipStream_t>(stream), "qk_norm_rope_hip");
 }
 
 extern "C" size_t qk_norm_rope_back_workspace_hip(const ppml_qk_norm_desc* a) {
     if (!desc_ok(a)) return 0;
     size_t most = 0;
-    for (const bool vec : {false, true}) {
-        const HeadPlan pl = plan_heads(*a, vec, true);
+    for (const int aligned : {1, 4, 8}) {
+        const HeadPlan pl = plan_heads(*a, aligned, true);
         const size_t bytes = static_cast<size_t>(pl.blocks) * pl.parts * 2 * static_cast<size_t>(a->d) * 4;
         if (bytes > most) most = bytes;
     }
@@ -440,11 +505,10 @@ extern "C" int qk_norm_rope_back_hip(const ppml_qk_norm_desc* a, const void* dq,
     p.side[0] = side_of(q, a->q_strides, dq, a->dq_strides, q_grad, a->q_out_strides, wq, a->hq);
     p.side[1] = side_of(k, a->k_strides, dk, a->dk_strides, k_grad, a->k_out_strides, wk, a->hk);
     p.partial = weights ? static_cast<float*>(workspace) : nullptr;
-    const size_t elem = elem_bytes(a->type);
-    const HeadPlan pl = plan_heads(*a, side_aligned(p.side[0], elem, true) && side_aligned(p.side[1], elem, true), true);
+    const HeadPlan pl = plan_heads(*a, both_aligned(p, elem_bytes(a->type), true), true);
     const int rc = run_heads(*a, p, pl, true, stream, "qk_norm_rope_back_hip");
     if (rc != RC_OK || !weights) return rc;
-    hipLaunchKernelGGL(head_norm_weights_kernel, dim3((a->d + 15) / 16, 2), dim3(256), 0, stream, static_cast<const float*>(workspace),
+    hipLaunchKernelGGL(head_norm_weights_kernel, dim3((a->d + 7) / 8, 2), dim3(256), 0, stream, static_cast<const float*>(workspace),
                        static_cast<int>(pl.blocks * pl.parts), a->d, wq_grad, wk_grad);
     return check_launch("qk_norm_rope_back_hip");
 }

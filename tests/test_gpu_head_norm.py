@@ -101,6 +101,9 @@ CASES = [
     (1, 4, 1, 1, 511, 510, False),
     (2, 3, 2, 2, 256, 192, False),
     (1, 700, 2, 2, 16, 8, False),
+    (1, 16400, 2, 1, 64, 64, False),    # sixteen-bit types eight elements at a time
+    (1, 33000, 1, 1, 48, 16, False),
+    (2, 8300, 1, 2, 64, 32, True),
     (1, 3000, 2, 1, 8, 8, False),       # work-groups of the backward pass that take several tokens each
 ]
 
