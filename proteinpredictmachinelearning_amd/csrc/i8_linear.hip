@@ -275,8 +275,8 @@ __device__ __forceinline__ void store_tokens(const I8Product& p, const Channels<
 template <class T>
 __device__ __forceinline__ bool whole_stores(const I8Product& p) { return p.w.rows % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0; }
 
-template <class T, class Loop>
-__global__ __launch_bounds__(Loop::THREADS, 2) void i8_product_kernel(const I8Product p) {
+template <class T, class Loop, bool DEEP>
+__global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 << 10 ? Loop::WAVES / 4 : 2) void i8_product_kernel(const I8Product p) {
     constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN, PITCH = TM * 16 + 4;
     __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
     __shared__ float x_scale[Loop::BN];
@@ -284,7 +284,12 @@ __global__ __launch_bounds__(Loop::THREADS, 2) void i8_product_kernel(const I8Pr
     const int m0 = (t % p.tiles_w) * Loop::BM, n0 = (t / p.tiles_w) * Loop::BN;
     for (int i = threadIdx.x; i < Loop::BN; i += Loop::THREADS) x_scale[i] = p.x_scale[n0 + i < p.x.rows ? n0 + i : p.x.rows - 1];
     v4i acc[TM][TN];
-    Loop::run(p.w, p.x, m0, n0, p.stages, even, odd, acc);
+    if constexpr (DEEP) {
+        __shared__ __attribute__((aligned(128))) uint8_t third[Loop::STAGE], fourth[Loop::STAGE];
+        Loop::run(p.w, p.x, m0, n0, p.stages, even, odd, third, fourth, acc);
+    } else {
+        Loop::run(p.w, p.x, m0, n0, p.stages, even, odd, acc);
+    }
     const int wave = threadIdx.x >> 6, nw = wave % WN * TN * 16;
     static_assert(Loop::WAVES / 2 * 16 * PITCH * 4 <= Loop::STAGE, "half of the waves' sixteen tokens fit a stage");
     __syncthreads();                                    // every wave has read its last stage
@@ -516,12 +521,12 @@ int launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, flo
     return check_launch(what);
 }
 
-template <class T, class Loop>
+template <class T, class Loop, bool DEEP>
 int launch_tiles(I8Product p, hipStream_t stream) {
     p.tiles_w = (p.w.rows + Loop::BM - 1) / Loop::BM;
     p.tiles_x = (p.x.rows + Loop::BN - 1) / Loop::BN;
     if (static_cast<int64_t>(p.tiles_w) * p.tiles_x > 0x7fffffff) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
-    hipLaunchKernelGGL((i8_product_kernel<T, Loop>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x)), dim3(Loop::THREADS), 0, stream, p);
+    hipLaunchKernelGGL((i8_product_kernel<T, Loop, DEEP>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x)), dim3(Loop::THREADS), 0, stream, p);
     return check_launch("mul_mat_i8_hip");
 }
 
@@ -571,9 +576,12 @@ int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* sca
     }
     const int rc = launch_quantize(rows, q, row, row, scale, stream, "mul_mat_i8_hip");
     if (rc != RC_OK) return rc;
-    const int64_t tiles256 = static_cast<int64_t>((p.w.rows + 255) / 256) * ((p.x.rows + 255) / 256);
-    if (tiles256 >= device_cu_count()) return launch_tiles<T, TilePingPong<StepI8>>(p, stream);
-    return launch_tiles<T, TileLoop<StepI8, 2, 2, 4, 4>>(p, stream);
+    const auto tiles = [&](int side) { return static_cast<double>((p.w.rows + side - 1) / side) * static_cast<double>((p.x.rows + static_cast<int64_t>(side) - 1) / side); };
+    switch (tile_side(tiles, 2.2)) {
+        case 256: return launch_tiles<T, TilePingPong<StepI8>, false>(p, stream);
+        case 128: return launch_tiles<T, TileDeep<StepI8, 2, 2, 4, 4>, true>(p, stream);
+        default:  return launch_tiles<T, TileDeep<StepI8, 2, 2, 2, 2>, true>(p, stream);
+    }
 }
 
 bool float_type(int type) { return type == PPML_ELEM_F32 || type == PPML_ELEM_F16 || type == PPML_ELEM_BF16; }

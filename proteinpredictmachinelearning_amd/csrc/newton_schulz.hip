@@ -16,6 +16,8 @@
 #include "elements.hpp"
 #include "tile_product.hpp"
 
+#include <type_traits>
+
 namespace ppmlhip {
 namespace {
 
@@ -120,14 +122,17 @@ __device__ __forceinline__ void put_operand(uint8_t* at, const float (&x)[16]) {
         *reinterpret_cast<v8h*>(at + 64 + 2 * o) = l;
     }
 }
-__device__ __forceinline__ void get_operand(const uint8_t* at, float (&x)[16]) {
+struct Operand16 {
+    v8h h[2], l[2];
+    __device__ __forceinline__ void fetch(const uint8_t* at) {
 #pragma unroll
-    for (int o = 0; o < 16; o += 8) {
-        const v8h h = *reinterpret_cast<const v8h*>(at + 2 * o), l = *reinterpret_cast<const v8h*>(at + 64 + 2 * o);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[o + e] = static_cast<float>(h[e]) + static_cast<float>(l[e]);
+        for (int o = 0; o < 2; ++o) {
+            h[o] = *reinterpret_cast<const v8h*>(at + 16 * o);
+            l[o] = *reinterpret_cast<const v8h*>(at + 64 + 16 * o);
+        }
     }
-}
+    __device__ __forceinline__ float value(int e) const { return static_cast<float>(h[e >> 3][e & 7]) + static_cast<float>(l[e >> 3][e & 7]); }
+};
 
 struct NsStart {
     const void* g;
@@ -238,9 +243,15 @@ __device__ __forceinline__ void ns_tile_of(const NsProduct& p, int& tm, int& tn)
 
 constexpr int NS_PITCH = 33;                            // floats from row to row of a block in LDS: rows and columns both meet different banks
 
+// What a lane adds to its half row of the block of 32 x 32 from (m0, n0) on
+__device__ __forceinline__ void ns_fetch_added(const NsProduct& p, Operand16& added, int64_t z, int m0, int n0) {
+    const int lane = threadIdx.x & 63, m = m0 + (lane >> 1), n = n0 + (lane & 1) * 16;
+    if (p.added && m < p.a.rows && n0 < p.b.rows) added.fetch(p.added + z * p.added_matrix + operand_at(m, p.added_stride, n));
+}
+
 // A block of 32 x 32 sums, in LDS, becomes what the launch writes: by rows (half a row per lane), with what is added, then by columns.
 template <class T>
-__device__ __forceinline__ void ns_finish_block(const NsProduct& p, float* lds, int64_t z, int m0, int n0, bool mirror, float of_sum, float of_added) {
+__device__ __forceinline__ void ns_finish_block(const NsProduct& p, float* lds, int64_t z, int m0, int n0, bool mirror, float of_sum, float of_added, const Operand16& added) {
     const int lane = threadIdx.x & 63, line = lane >> 1, part = (lane & 1) * 16;
     const int M = p.a.rows, N = p.b.rows;
     T* const final = p.final ? static_cast<T*>(p.final) + z * p.final_matrix : nullptr;
@@ -261,10 +272,8 @@ __device__ __forceinline__ void ns_finish_block(const NsProduct& p, float* lds, 
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = row[e] * of_sum;
         if (p.added && m < M && n0 < N) {
-            float y[16];
-            get_operand(p.added + z * p.added_matrix + operand_at(m, p.added_stride, n), y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = fmaf(y[e], of_added, x[e]);
+            for (int e = 0; e < 16; ++e) x[e] = fmaf(added.value(e), of_added, x[e]);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -290,8 +299,8 @@ __device__ __forceinline__ void ns_finish_block(const NsProduct& p, float* lds, 
     }
 }
 
-template <class T, class Loop>
-__global__ __launch_bounds__(Loop::THREADS, 2) void ns_product_kernel(const NsProduct p) {
+template <class T, class Loop, bool DEEP>
+__global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 << 10 ? Loop::WAVES / 4 : 2) void ns_product_kernel(const NsProduct p) {
     constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN;
     __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
     const int64_t z = blockIdx.y;
@@ -302,17 +311,25 @@ __global__ __launch_bounds__(Loop::THREADS, 2) void ns_product_kernel(const NsPr
     A.base += z * p.a_matrix;
     B.base += z * p.b_matrix;
     v4f acc[TM][TN];
-    Loop::run(A, B, m0, n0, p.stages, even, odd, acc);
+    if constexpr (DEEP) {
+        __shared__ __attribute__((aligned(128))) uint8_t third[Loop::STAGE], fourth[Loop::STAGE];
+        Loop::run(A, B, m0, n0, p.stages, even, odd, third, fourth, acc);
+    } else {
+        Loop::run(A, B, m0, n0, p.stages, even, odd, acc);
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float of_sum = p.factors[z].of_sum[p.which], of_added = p.factors[z].of_added[p.which];
-    static_assert(Loop::WAVES * 32 * NS_PITCH * 4 <= Loop::STAGE, "a block per wave fits a stage");
+    static_assert(Loop::WAVES / 2 * 32 * NS_PITCH * 4 <= Loop::STAGE, "a block for half of the waves fits a stage");
     __syncthreads();                                    // every wave has read its last stage
-    float* const lds = reinterpret_cast<float*>(even) + wave * 32 * NS_PITCH;
+    float* const lds = reinterpret_cast<float*>(wave & 1 ? odd : even) + (wave >> 1) * 32 * NS_PITCH;
     const bool mirror = p.symmetric && tm != tn;
 #pragma unroll
     for (int i = 0; i < TM; i += 2)
 #pragma unroll
         for (int j = 0; j < TN; j += 2) {
+            const int mb = m0 + (wave / WN * TM + i) * 16, nb = n0 + (wave % WN * TN + j) * 16;
+            Operand16 added{};
+            ns_fetch_added(p, added, z, mb, nb);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -320,43 +337,9 @@ __global__ __launch_bounds__(Loop::THREADS, 2) void ns_product_kernel(const NsPr
 #pragma unroll
                     for (int r = 0; r < 4; ++r) lds[(16 * u + (lane >> 4) * 4 + r) * NS_PITCH + 16 * v + (lane & 15)] = acc[i + u][j + v][r];
             wave_fence();
-            ns_finish_block<T>(p, lds, z, m0 + (wave / WN * TM + i) * 16, n0 + (wave % WN * TN + j) * 16, mirror, of_sum, of_added);
+            ns_finish_block<T>(p, lds, z, mb, nb, mirror, of_sum, of_added, added);
             wave_fence();
         }
-}
-
-// A tile of 32 x 32 per work-group, its waves each a share of K
-template <class T, int WAVES, int DEEP>
-__global__ __launch_bounds__(WAVES * 64) void ns_small_kernel(const NsProduct p) {
-    typedef TileSplit<StepF16x2, WAVES, 2, 2, DEEP> Split;
-    __shared__ float lds[WAVES][32 * NS_PITCH];
-    const int64_t z = blockIdx.y;
-    int tm, tn;
-    ns_tile_of(p, tm, tn);
-    const int m0 = tm * Split::BM, n0 = tn * Split::BN;
-    RowBytes A = p.a, B = p.b;
-    A.base += z * p.a_matrix;
-    B.base += z * p.b_matrix;
-    v4f acc[2][2];
-    Split::run(A, B, m0, n0, p.stages, acc);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float of_sum = p.factors[z].of_sum[p.which], of_added = p.factors[z].of_added[p.which];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) lds[wave][(16 * u + (lane >> 4) * 4 + r) * NS_PITCH + 16 * v + (lane & 15)] = acc[u][v][r];
-    __syncthreads();
-    for (int i = tid; i < 32 * 32; i += WAVES * 64) {
-        const int at = (i >> 5) * NS_PITCH + (i & 31);
-        float sum = lds[0][at];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) sum += lds[w][at];
-        lds[0][at] = sum;
-    }
-    __syncthreads();
-    if (wave == 0) ns_finish_block<T>(p, lds[0], z, m0, n0, p.symmetric && tm != tn, of_sum, of_added);
 }
 
 // ------------------------------------------------------------------------------------------------------------ host side
@@ -398,6 +381,11 @@ bool ns_fits(int64_t batch, int64_t rows, int64_t cols) {
     return batch > 0 && batch <= 65535 && rows > 0 && cols > 0 && rows <= NS_MOST_SIDE && cols <= NS_MOST_SIDE;
 }
 
+int64_t ns_tiles(const NsProduct& p, int side) {
+    const int64_t m = (p.a.rows + side - 1) / side, n = (p.b.rows + side - 1) / side;
+    return p.symmetric ? n * (n + 1) / 2 : m * n;
+}
+
 template <class T>
 int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int64_t cols, int steps, const NsCoefficients& k, float eps, uint8_t* ws,
                       hipStream_t stream) {
@@ -421,22 +409,17 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
     const auto product = [&](NsProduct p) {
         p.factors = factors;
         p.final_vec = out_vec;
-        const auto tiles = [&](int side) {
-            p.tiles_m = (p.a.rows + side - 1) / side;
-            p.tiles_n = (p.b.rows + side - 1) / side;
-            return p.symmetric ? static_cast<int64_t>(p.tiles_n) * (p.tiles_n + 1) / 2 : static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+        const auto launch = [&](auto loop, auto deep) {
+            typedef decltype(loop) Loop;
+            p.tiles_m = (p.a.rows + Loop::BM - 1) / Loop::BM;
+            p.tiles_n = (p.b.rows + Loop::BN - 1) / Loop::BN;
+            hipLaunchKernelGGL((ns_product_kernel<T, Loop, decltype(deep)::value>), dim3(static_cast<unsigned>(ns_tiles(p, Loop::BM)), static_cast<unsigned>(batch)),
+                               dim3(Loop::THREADS), 0, stream, p);
         };
-        if (tiles(128) * batch < device_cu_count()) {
-            const dim3 grid(static_cast<unsigned>(tiles(32)), static_cast<unsigned>(batch));
-            if (p.stages > 4) hipLaunchKernelGGL((ns_small_kernel<T, 8, 3>), grid, dim3(512), 0, stream, p);
-            else              hipLaunchKernelGGL((ns_small_kernel<T, 4, 1>), grid, dim3(256), 0, stream, p);
-        } else {
-            typedef TileLoop<StepF16x2, 2, 2, 4, 4> Loop;
-            typedef TilePingPong<StepF16x2> Large;
-            if (tiles(256) * batch >= device_cu_count())
-                hipLaunchKernelGGL((ns_product_kernel<T, Large>), dim3(static_cast<unsigned>(tiles(256)), static_cast<unsigned>(batch)), dim3(Large::THREADS), 0, stream, p);
-            else
-                hipLaunchKernelGGL((ns_product_kernel<T, Loop>), dim3(static_cast<unsigned>(tiles(128)), static_cast<unsigned>(batch)), dim3(Loop::THREADS), 0, stream, p);
+        switch (tile_side([&](int side) { return static_cast<double>(ns_tiles(p, side)) * static_cast<double>(batch); }, 2.55)) {
+            case 256: launch(TilePingPong<StepF16x2>{}, std::false_type{}); break;
+            case 128: launch(TileDeep<StepF16x2, 2, 2, 4, 4>{}, std::true_type{}); break;
+            default:  launch(TileDeep<StepF16x2, 2, 2, 2, 2>{}, std::true_type{}); break;
         }
     };
     const int m = static_cast<int>(l.m), n = static_cast<int>(l.n);

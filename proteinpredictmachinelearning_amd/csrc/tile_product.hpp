@@ -3,6 +3,8 @@
 #pragma once
 #include "split.hpp"
 
+#include <cmath>
+
 namespace ppmlhip {
 
 // A dense operand: rows of bytes along k, zero from the last k on to a whole number of 128.
@@ -22,6 +24,17 @@ typedef __attribute__((address_space(3))) void* lds_void;
 __device__ __forceinline__ void load_to_lds(const __amdgpu_buffer_rsrc_t& rsrc, uint8_t* to, uint32_t voffset, uint32_t soffset) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void)to, 16, voffset, soffset, 0, 0);
+#endif
+}
+
+// A barrier that nothing moves past and that waits for nothing by itself
+__device__ __forceinline__ void bare_barrier() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
 #endif
 }
 
@@ -58,27 +71,31 @@ __device__ __forceinline__ void step_tiles(const v4i (&a)[TM][2], const v4i (&b)
     if constexpr (TERM + 1 < Step::TERMS) step_tiles<Step, TERM + 1>(a, b, acc);
 }
 
-// WM x WN waves, each with TM x TN tiles of 16 x 16.  In lane l, register r of acc[i][j] holds the product of A's row
+// A tile of the product: WM x WN waves, each with TM x TN tiles of 16 x 16.  In lane l, register r of acc[i][j] holds the product of A's row
 // m0 + (wave's first) + 16 i + 4 (l / 16) + r and B's row n0 + (wave's first) + 16 j + l % 16.
 //
 // A row's 128 bytes lie in LDS as eight pieces of sixteen, piece p of row r in place p ^ (r / 2 & 7): sixteen lanes that read the
-// same piece of sixteen rows meet all 64 banks once.  The loads to LDS put lane l's piece at place l, so it is the address that a lane
-// loads from which is permuted.
+// same piece of sixteen rows meet all 64 banks once.  The loads to LDS put lane l's piece at place l, so it is the address that a
+// lane loads from which is permuted.
+//
+// The stages' LDS arrays are the kernel's, each of STAGE bytes, aligned to 128 and declared by itself: the compiler tells loads from one from
+// stores to another by their names, and lets the former pass loads to LDS that are still on their way to the latter.
+//
+// TileDeep: three stages are on their way while one is contracted (four arrays).  A work-group of a product of few tiles has a CU to itself and
+// nothing else to do while a stage travels: with one on its way (two arrays) 1024 x 1024 x 1024 in two halves took 24 us instead of 12 in tiles of 64 x 64.
 template <class Step, int WM_, int WN_, int TM_, int TN_>
-struct TileLoop {
+struct TileDeep {
     static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_;
     static constexpr int BM = WM * TM * 16, BN = WN * TN * 16, WAVES = WM * WN, THREADS = WAVES * 64;
     static constexpr int STAGE = (BM + BN) * TILE_K;
-    static constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES;      // a load fetches eight rows
+    static constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, LOADS = LOADS_A + LOADS_B;      // a load fetches eight rows
     static_assert(WAVES % 2 == 0 && BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole loads per wave");
     typedef typename Step::Acc Acc;
 
-    // `even` and `odd` are LDS arrays of their own, of STAGE bytes each and aligned to 128: the compiler tells loads from the one from
-    // stores to the other by their names, and lets the former pass loads to LDS that are still on their way to the latter.
-    __device__ static __forceinline__ void run(const RowBytes& A, const RowBytes& B, int m0, int n0, int stages, uint8_t* even, uint8_t* odd, Acc (&acc)[TM][TN]) {
+    __device__ static __forceinline__ void run(const RowBytes& A, const RowBytes& B, int m0, int n0, int stages, uint8_t* s0, uint8_t* s1, uint8_t* s2, uint8_t* s3,
+                                               Acc (&acc)[TM][TN]) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wm = wave / WN, wn = wave % WN;
-        // (rows behind the last one are that row again: their products are nobody's)
         const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A.base + m0 * A.stride), 0, 0x7fffffff, 0x00020000);
         const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B.base + n0 * B.stride), 0, 0x7fffffff, 0x00020000);
         const int row8 = lane >> 3, piece = (lane & 7) ^ (4 * (wave & 1) + (row8 >> 1));
@@ -93,16 +110,30 @@ struct TileLoop {
             const int r = (i * WAVES + wave) * 8 + row8, last = B.rows - 1 - n0;
             from_b[i] = static_cast<uint32_t>((r < last ? r : last) * B.stride) + piece * 16u;
         }
+        // (past the last stage that one again, into an array nobody reads: as many loads are on their way in every iteration)
         const auto request = [&](uint8_t* to, int stage) {
+            const int at = (stage < stages ? stage : stages - 1) * TILE_K;
 #pragma unroll
-            for (int i = 0; i < LOADS_A; ++i) load_to_lds(ra, to + (i * WAVES + wave) * 8 * TILE_K, from_a[i], stage * TILE_K);
+            for (int i = 0; i < LOADS_A; ++i) load_to_lds(ra, to + (i * WAVES + wave) * 8 * TILE_K, from_a[i], at);
 #pragma unroll
-            for (int i = 0; i < LOADS_B; ++i) load_to_lds(rb, to + (BM + (i * WAVES + wave) * 8) * TILE_K, from_b[i], stage * TILE_K);
+            for (int i = 0; i < LOADS_B; ++i) load_to_lds(rb, to + (BM + (i * WAVES + wave) * 8) * TILE_K, from_b[i], at);
         };
         const int lane_at[2] = {(lane & 15) * TILE_K + (((lane >> 4) ^ ((lane & 15) >> 1)) * 16), (lane & 15) * TILE_K + (((4 + (lane >> 4)) ^ ((lane & 15) >> 1)) * 16)};
-        const auto contract = [&](const uint8_t* from) {
-            const uint8_t* const a_at = from + wm * TM * 16 * TILE_K;
-            const uint8_t* const b_at = from + (BM + wn * TN * 16) * TILE_K;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = Acc{};
+        // One barrier per stage: behind it the stage is in LDS (every wave has waited for its own part), and the one before has been read.
+        const auto stage = [&](const uint8_t* here, uint8_t* free, int s) {
+            static_assert(LOADS == 4 || LOADS == 8, "the wait below names 2 LOADS");
+#if defined(__HIP_DEVICE_COMPILE__)
+            if constexpr (LOADS == 4) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            else                      asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+#endif
+            bare_barrier();
+            request(free, s + 3);
+            const uint8_t* const a_at = here + wm * TM * 16 * TILE_K;
+            const uint8_t* const b_at = here + (BM + wn * TN * 16) * TILE_K;
             v4i a[TM][2], b[TN][2];
 #pragma unroll
             for (int i = 0; i < TM; ++i)
@@ -114,25 +145,23 @@ struct TileLoop {
                 for (int h = 0; h < 2; ++h) b[j][h] = *reinterpret_cast<const v4i*>(b_at + j * 16 * TILE_K + lane_at[h]);
             step_tiles<Step>(a, b, acc);
         };
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = Acc{};
-        // A barrier says both "the stage is in LDS" (it waits for the loads) and "the one before has been read".
-        request(even, 0);
-        int stage = 0;
-        for (; stage + 2 <= stages; stage += 2) {
-            __syncthreads();
-            request(odd, stage + 1);
-            contract(even);
-            __syncthreads();
-            if (stage + 2 < stages) request(even, stage + 2);
-            contract(odd);
+        request(s0, 0);
+        request(s1, 1);
+        request(s2, 2);
+        int s = 0;
+#pragma unroll 1
+        for (; s + 4 <= stages; s += 4) {
+            stage(s0, s3, s);
+            stage(s1, s0, s + 1);
+            stage(s2, s1, s + 2);
+            stage(s3, s2, s + 3);
         }
-        if (stage < stages) {
-            __syncthreads();
-            contract(even);
-        }
+        if (s < stages) stage(s0, s3, s);
+        if (s + 1 < stages) stage(s1, s0, s + 1);
+        if (s + 2 < stages) stage(s2, s1, s + 2);
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (nothing is on its way to LDS when the caller uses it)
+#endif
     }
 };
 
@@ -157,17 +186,6 @@ struct TilePingPong {
         const int left = x.rows - first < BM ? x.rows - first : BM;
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x.base + first * x.stride), 0, static_cast<int>(left * x.stride), 0x00020000);
     }
-    // (nothing moves past it; the compiler puts no wait in front of it either)
-    __device__ static __forceinline__ void barrier() {
-#if defined(__HIP_DEVICE_COMPILE__)
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("" ::: "memory");
-#endif
-    }
-
     __device__ static __forceinline__ void run(const RowBytes& A, const RowBytes& B, int m0, int n0, int stages, uint8_t* even, uint8_t* odd, Acc (&acc)[TM][TN]) {
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wm = wave / WN, wn = wave % WN;       // wm: the group
@@ -217,16 +235,16 @@ struct TilePingPong {
             for (int j = 0; j < TN; ++j) acc[i][j] = Acc{};
         request(even, 0);
         wait_loads();
-        barrier();
+        bare_barrier();
         if (wm == 0) {
             const auto stage = [&](uint8_t* here, uint8_t* next, int s) {
                 if (s + 1 < stages) request(next, s + 1);
                 read(here);
                 wait_lds();
-                barrier();
+                bare_barrier();
                 contract();
                 wait_loads();
-                barrier();
+                bare_barrier();
             };
             int s = 0;
 #pragma unroll 1
@@ -239,11 +257,11 @@ struct TilePingPong {
             const auto stage = [&](uint8_t* here, uint8_t* next, int s) {
                 if (s + 1 < stages) request(next, s + 1);
                 if (s > 0) contract();
-                barrier();
+                bare_barrier();
                 read(here);
                 wait_lds();
                 wait_loads();
-                barrier();
+                bare_barrier();
             };
             int s = 0;
 #pragma unroll 1
@@ -257,56 +275,16 @@ struct TilePingPong {
     }
 };
 
-// Few tiles: one tile of 16 TM x 16 TN per work-group, its WAVES waves take every WAVES-th stage each, straight from memory to registers.
-// What bounds a small product is the way to memory and back, and all of a wave's stages travel it together (DEEP at a time).
-// The waves' sums are the caller's to add.
-template <class Step, int WAVES, int TM, int TN, int DEEP>
-struct TileSplit {
-    static constexpr int BM = TM * 16, BN = TN * 16, THREADS = WAVES * 64;
-    typedef typename Step::Acc Acc;
-
-    __device__ static __forceinline__ void run(const RowBytes& A, const RowBytes& B, int m0, int n0, int stages, Acc (&acc)[TM][TN]) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A.base + m0 * A.stride), 0, 0x7fffffff, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B.base + n0 * B.stride), 0, 0x7fffffff, 0x00020000);
-        uint32_t from_a[TM], from_b[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int r = 16 * i + (lane & 15), last = A.rows - 1 - m0;
-            from_a[i] = static_cast<uint32_t>((r < last ? r : last) * A.stride) + (lane >> 4) * 16u;
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int r = 16 * j + (lane & 15), last = B.rows - 1 - n0;
-            from_b[j] = static_cast<uint32_t>((r < last ? r : last) * B.stride) + (lane >> 4) * 16u;
-        }
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = Acc{};
-        const auto load = [](const __amdgpu_buffer_rsrc_t& r, uint32_t at, int stage, int h) {
-            return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, at, stage * TILE_K + h * 64, 0));
-        };
-        for (int first = wave; first < stages; first += WAVES * DEEP) {
-            v4i a[DEEP][TM][2], b[DEEP][TN][2];
-#pragma unroll
-            for (int d = 0; d < DEEP; ++d) {
-                // (a stage behind the last one is loaded again and not used)
-                const int stage = first + d * WAVES < stages ? first + d * WAVES : first;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) a[d][i][h] = load(ra, from_a[i], stage, h);
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) b[d][j][h] = load(rb, from_b[j], stage, h);
-                }
-            }
-#pragma unroll
-            for (int d = 0; d < DEEP; ++d)
-                if (first + d * WAVES < stages) step_tiles<Step>(a[d], b[d], acc);
-        }
-    }
-};
+// Tiles of 256 (TilePingPong), 128 or 64 (TileDeep) a side: whichever is done first.  A round of them over the CUs takes, per stage: `large`, 0.78 and
+// 0.32 us (measured: in two halves 4096 x 4096 x 4096 327 us with 256 a side and 397 with 128, 2048 x 2048 x 2048 138, 54 and 81 with 64, 1024 x 1024 x 1024
+// symmetric 24 with 128 and 12 with 64; in 8-bit integers over 4096, N tokens onto 4096 channels, quantizer included: N = 256 55, 26 and 19,
+// 1024 60, 33 and 49, 4096 85, 115 and 174).  Two work-groups of the smallest share a CU, so that a part of a round is not a whole one.
+template <class Tiles>
+int tile_side(const Tiles& tiles, double large) {
+    const double cus = device_cu_count();
+    const double t256 = large * std::ceil(tiles(256) / cus), t128 = 0.78 * std::ceil(tiles(128) / cus), t64 = 0.32 * std::fmax(1.0, tiles(64) / cus);
+    return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+}
 
 }  // namespace
 }  // namespace ppmlhip
