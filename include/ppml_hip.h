@@ -422,8 +422,9 @@ size_t i8_weight_row_bytes_hip(int K);
 int i8_weight_pack_hip(const int8_t *w, int64_t w_stride, int M, int K, int8_t *packed, ppml_hip_stream_t stream);
 /* y[n * M + m] = (sum_k q[n][k] w[m][k]) * x_scale[n] * w_scale[m] + (bias ? bias[m] : 0), rounded to y_type (F32, F16 or BF16).  x (N x K, x_stride elements
  * apart) is F32, F16 or BF16 and quantized by the rule above on the way (x_scale is not read), or I8 with its x_scale.  The sums are exact.  M <= 2^22.  A token
- * whose scale is NaN is NaN throughout.  The workspace, mul_mat_i8_workspace_hip(N, K) bytes, 16-byte aligned, is the call's until its work has run. */
-size_t mul_mat_i8_workspace_hip(int N, int K);
+ * whose scale is NaN is NaN throughout.  The workspace, mul_mat_i8_workspace_hip(M, N, K) bytes (0: NULL will do), 16-byte aligned, is the call's until its work
+ * has run. */
+size_t mul_mat_i8_workspace_hip(int M, int N, int K);
 int mul_mat_i8_hip(const int8_t *packed, const float *w_scale, const void *x, int x_type, int64_t x_stride, const float *x_scale, const float *bias,
                    void *y, int y_type, int M, int N, int K, void *workspace, size_t workspace_bytes, ppml_hip_stream_t stream);
 

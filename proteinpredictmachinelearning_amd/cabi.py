@@ -53,7 +53,7 @@ SIGNATURES = {
     "quantize_rows_i8_hip": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i64, _i, _vp]),
     "i8_weight_row_bytes_hip": (C.c_size_t, [_i]),
     "i8_weight_pack_hip": (_i, [_vp, _i64, _i, _i, _vp, _vp]),
-    "mul_mat_i8_workspace_hip": (C.c_size_t, [_i, _i]),
+    "mul_mat_i8_workspace_hip": (C.c_size_t, [_i, _i, _i]),
     "mul_mat_i8_hip": (_i, [_vp, _vp, _vp, _i, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp, C.c_size_t, _vp]),
     "qk_norm_rope_hip": (_i, [_vp] * 10),
     "qk_norm_rope_back_workspace_hip": (C.c_size_t, [_vp]),

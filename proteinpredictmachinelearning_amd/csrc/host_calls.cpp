@@ -21,11 +21,15 @@
 #include <cstdint>
 #include <cstring>
 
+#include "../../include/ppml_hip.h"
+
 namespace {
 
-enum Launcher { MUL_MAT, MUL_MAT_F16, MUL_MAT_Q8, MUL_MAT_Q8_EX, OPM, OPM_BACK, TRI_MUL, TRI_MUL_BACK, ATTN, ATTN_BACK, LAUNCHERS };
+enum Launcher { MUL_MAT, MUL_MAT_F16, MUL_MAT_Q8, MUL_MAT_Q8_EX, OPM, OPM_BACK, TRI_MUL, TRI_MUL_BACK, ATTN, ATTN_BACK, I8, I8_WS, QK, QK_BACK, QK_BACK_WS, NS, NS_WS, LAUNCHERS };
 const char* const LAUNCHER_NAMES[LAUNCHERS] = {"mul_mat_hip", "mul_mat_f16_hip", "mul_mat_q8_hip", "mul_mat_q8_ex_hip", "outer_prod_mean_hip", "outer_prod_mean_back_hip",
-                                               "tri_mul_hip", "tri_mul_back_hip", "flash_attn_forward_ex_hip", "flash_attn_backward_hip"};
+                                               "tri_mul_hip", "tri_mul_back_hip", "flash_attn_forward_ex_hip", "flash_attn_backward_hip", "mul_mat_i8_hip",
+                                               "mul_mat_i8_workspace_hip", "qk_norm_rope_hip", "qk_norm_rope_back_hip", "qk_norm_rope_back_workspace_hip", "newton_schulz_hip",
+                                               "newton_schulz_workspace_hip"};
 void* g_launcher[LAUNCHERS];
 std::atomic<uint64_t> g_ready{0};                       // a bit per device
 
@@ -43,17 +47,24 @@ struct Call {
         ordinary = i >= 0 && i < 64 && (g_ready.load(std::memory_order_acquire) >> i & 1) != 0 && guard.getStream(device).id() == 0 &&
                    !at::impl::torch_function_mode_enabled() && !c10::impl::TorchDispatchModeTLS::any_modes_set();
     }
-    // `obj` as a tensor of this call (a null pointer for None where that is allowed)
-    const Tensor* tensor(PyObject* obj, at::ScalarType type, bool optional = false) {
+    // `obj` as a tensor of this call, of any type and strides (a null pointer for None where that is allowed)
+    const Tensor* any(PyObject* obj, bool optional = false) {
         static const c10::DispatchKeySet plain({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
         if (!ordinary || (optional && obj == Py_None)) return nullptr;
         if (!THPVariable_CheckExact(obj)) { ordinary = false; return nullptr; }
         const Tensor& t = THPVariable_Unpack(obj);
-        ordinary = t.defined() && (t.key_set().raw_repr() & ~plain.raw_repr()) == 0 && t.layout() == at::kStrided && t.scalar_type() == type && t.device() == device &&
-                   t.is_contiguous() && !t.is_conj() && !t.is_neg();
+        ordinary = t.defined() && (t.key_set().raw_repr() & ~plain.raw_repr()) == 0 && t.layout() == at::kStrided && t.device() == device && !t.is_conj() && !t.is_neg();
         return ordinary ? &t : nullptr;
     }
-    Tensor empty(at::IntArrayRef sizes) const { return at::empty(sizes, at::TensorOptions().dtype(at::kFloat).device(device)); }
+    // ... of this type, contiguous
+    const Tensor* tensor(PyObject* obj, at::ScalarType type, bool optional = false) {
+        const Tensor* const t = any(obj, optional);
+        if (t) ordinary = t->scalar_type() == type && t->is_contiguous();
+        return t && ordinary ? t : nullptr;
+    }
+    Tensor empty(at::IntArrayRef sizes, at::ScalarType type = at::kFloat) const { return at::empty(sizes, at::TensorOptions().dtype(type).device(device)); }
+    // (at::empty of bytes: null for none)
+    Tensor bytes(size_t n) const { return n ? empty({static_cast<int64_t>(n)}, at::kByte) : Tensor(); }
 };
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -259,6 +270,139 @@ PyObject* flash_attn_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// the launchers' element types; -1: none of them
+int elem(at::ScalarType t) { return t == at::kFloat ? PPML_ELEM_F32 : t == at::kHalf ? PPML_ELEM_F16 : t == at::kBFloat16 ? PPML_ELEM_BF16 : t == at::kChar ? PPML_ELEM_I8 : -1; }
+constexpr at::ScalarType ELEM_SCALARS[3] = {at::kFloat, at::kHalf, at::kBFloat16};
+void* raw(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+const void* raw(const Tensor* t) { return t ? t->const_data_ptr() : nullptr; }
+
+// (packed weight, its scales, K, x, x's scales or None, bias or None, type of the result or -1: x's)
+PyObject* mul_mat_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        int64_t K, type;
+        if (n != 7 || !integer(args[2], K) || K <= 0 || !fits(K) || !integer(args[6], type) || type > PPML_ELEM_BF16) return none();
+        Call call;
+        const Tensor *w = call.tensor(args[0], at::kChar), *ws = call.tensor(args[1], at::kFloat), *x = call.any(args[3]), *xs = call.tensor(args[4], at::kFloat, true),
+                     *bias = call.tensor(args[5], at::kFloat, true);
+        if (!call.ordinary || x->dim() != 2 || x->size(1) != K || !x->is_contiguous() || w->dim() != 2 || ws->dim() != 1 || ws->size(0) != w->size(0)) return none();
+        const int64_t N = x->size(0), M = w->size(0);
+        const int x_type = elem(x->scalar_type());
+        if (N <= 0 || M <= 0 || !fits(N) || !fits(M) || x_type < 0 || (x_type == PPML_ELEM_I8) != (xs != nullptr) || (xs && (xs->dim() != 1 || xs->size(0) != N)) ||
+            (bias && (bias->dim() != 1 || bias->size(0) != M))) return none();
+        const int y_type = type >= 0 ? static_cast<int>(type) : x_type == PPML_ELEM_I8 ? static_cast<int>(PPML_ELEM_F32) : x_type;
+        const int m = static_cast<int>(M), t = static_cast<int>(N), k = static_cast<int>(K);
+        Tensor y = call.empty({N, M}, ELEM_SCALARS[y_type]);
+        const size_t need = reinterpret_cast<size_t (*)(int, int, int)>(g_launcher[I8_WS])(m, t, k);
+        Tensor space = call.bytes(need);
+        const int rc = launch<const int8_t*, cf, cv, int, int64_t, cf, cf, void*, int, int, int, int, void*, size_t, void*>(
+            I8, static_cast<const int8_t*>(raw(w)), f(ws), raw(x), x_type, K, f(xs), f(bias), raw(y), y_type, m, t, k, raw(space), need, nullptr);
+        return rc == 0 ? wrap(std::move(y)) : none();
+    });
+}
+
+// What qk_norm_rope and its backward share: (q, k, wq, wk, freqs, positions, eps, interleaved) from args[0] on
+struct QkCall {
+    ppml_qk_norm_desc a{};
+    const Tensor *q = nullptr, *k = nullptr, *wq = nullptr, *wk = nullptr, *freqs = nullptr, *positions = nullptr;
+
+    static void steps(int64_t (&to)[3], const Tensor& t, int b, int l, int h) {
+        const int dims[3] = {b, l, h};
+        for (int i = 0; i < 3; ++i) to[i] = t.size(dims[i]) > 1 ? t.stride(dims[i]) : 0;
+    }
+    static bool heads(const Tensor& t) { return t.dim() == 4 && t.numel() > 0 && (t.size(3) == 1 || t.stride(3) == 1); }
+
+    bool take(Call& call, PyObject* const* args) {
+        double eps;
+        int64_t interleaved;
+        if (!number(args[6], eps) || !(eps >= 0.0) || !integer(args[7], interleaved)) return false;
+        q = call.any(args[0]); k = call.any(args[1]);
+        wq = call.tensor(args[2], at::kFloat, true); wk = call.tensor(args[3], at::kFloat, true);
+        freqs = call.tensor(args[4], at::kDouble, true); positions = call.any(args[5], true);
+        if (!call.ordinary || !heads(*q) || !heads(*k) || q->scalar_type() != k->scalar_type() || elem(q->scalar_type()) < 0 || elem(q->scalar_type()) == PPML_ELEM_I8) return false;
+        const int64_t B = q->size(0), L = q->size(1), d = q->size(3);
+        if (k->size(0) != B || k->size(1) != L || k->size(3) != d || d > 512 || q->size(2) > 65535 || k->size(2) > 65535) return false;
+        for (const Tensor* w : {wq, wk}) if (w && (w->dim() != 1 || w->size(0) != d)) return false;
+        if (freqs && (freqs->dim() != 1 || 2 * freqs->size(0) > d)) return false;
+        a.B = B; a.L = L; a.d = static_cast<int32_t>(d);
+        a.hq = static_cast<int32_t>(q->size(2)); a.hk = static_cast<int32_t>(k->size(2));
+        a.rot = freqs ? static_cast<int32_t>(2 * freqs->size(0)) : 0;
+        a.type = elem(q->scalar_type()); a.interleaved = interleaved ? 1 : 0; a.eps = static_cast<float>(eps);
+        if (positions) {
+            const bool shared = positions->dim() == 1 && positions->size(0) == L, each = positions->dim() == 2 && positions->size(0) == B && positions->size(1) == L;
+            const at::ScalarType type = positions->scalar_type();
+            if ((!shared && !each) || !positions->is_contiguous() || (type != at::kInt && type != at::kLong)) return false;
+            a.position_bytes = type == at::kInt ? 4 : 8;
+            a.position_stride = each ? L : 0;
+        }
+        steps(a.q_strides, *q, 0, 1, 2);
+        steps(a.k_strides, *k, 0, 1, 2);
+        return true;
+    }
+};
+
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 8) return none();
+        Call call;
+        QkCall c;
+        if (!c.take(call, args)) return none();
+        Tensor yq = call.empty({c.a.B, c.a.hq, c.a.L, c.a.d}, c.q->scalar_type()), yk = call.empty({c.a.B, c.a.hk, c.a.L, c.a.d}, c.q->scalar_type());
+        QkCall::steps(c.a.q_out_strides, yq, 0, 2, 1);
+        QkCall::steps(c.a.k_out_strides, yk, 0, 2, 1);
+        const int rc = launch<const ppml_qk_norm_desc*, cv, cv, cf, cf, const double*, cv, void*, void*, void*>(
+            QK, &c.a, raw(c.q), raw(c.k), f(c.wq), f(c.wk), static_cast<const double*>(raw(c.freqs)), raw(c.positions), raw(yq), raw(yk), nullptr);
+        return rc == 0 ? Py_BuildValue("(NN)", wrap(std::move(yq)), wrap(std::move(yk))) : none();
+    });
+}
+
+// (dq, dk, then as above): gradients in memory of their own
+PyObject* qk_norm_rope_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 10) return none();
+        Call call;
+        QkCall c;
+        if (!c.take(call, args + 2)) return none();
+        const Tensor *dq = call.any(args[0]), *dk = call.any(args[1]);
+        if (!call.ordinary || dq->scalar_type() != c.q->scalar_type() || dk->scalar_type() != c.q->scalar_type() || !QkCall::heads(*dq) || !QkCall::heads(*dk) ||
+            dq->sizes() != at::IntArrayRef({c.a.B, c.a.hq, c.a.L, c.a.d}) || dk->sizes() != at::IntArrayRef({c.a.B, c.a.hk, c.a.L, c.a.d})) return none();
+        QkCall::steps(c.a.dq_strides, *dq, 0, 2, 1);
+        QkCall::steps(c.a.dk_strides, *dk, 0, 2, 1);
+        Tensor gq = call.empty({c.a.B, c.a.L, c.a.hq, c.a.d}, c.q->scalar_type()), gk = call.empty({c.a.B, c.a.L, c.a.hk, c.a.d}, c.q->scalar_type()), gwq, gwk;
+        QkCall::steps(c.a.q_out_strides, gq, 0, 1, 2);
+        QkCall::steps(c.a.k_out_strides, gk, 0, 1, 2);
+        if (c.wq) gwq = call.empty({c.a.d});
+        if (c.wk) gwk = call.empty({c.a.d});
+        const size_t need = c.wq || c.wk ? reinterpret_cast<size_t (*)(const ppml_qk_norm_desc*)>(g_launcher[QK_BACK_WS])(&c.a) : 0;
+        Tensor space = call.bytes(need);
+        const int rc = launch<const ppml_qk_norm_desc*, cv, cv, cv, cv, cf, cf, const double*, cv, void*, void*, float*, float*, void*, size_t, void*>(
+            QK_BACK, &c.a, raw(dq), raw(dk), raw(c.q), raw(c.k), f(c.wq), f(c.wk), static_cast<const double*>(raw(c.freqs)), raw(c.positions), raw(gq), raw(gk), f(gwq), f(gwk),
+            raw(space), need, nullptr);
+        return rc == 0 ? Py_BuildValue("(NNNN)", wrap(std::move(gq)), wrap(std::move(gk)), wrap_or_none(std::move(gwq)), wrap_or_none(std::move(gwk))) : none();
+    });
+}
+
+// (g, steps, a, b, c, eps)
+PyObject* newton_schulz(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        int64_t steps;
+        double k[4];
+        if (n != 6 || !integer(args[1], steps) || steps < 1 || steps > 32) return none();
+        for (int i = 0; i < 4; ++i) if (!number(args[2 + i], k[i])) return none();
+        Call call;
+        const Tensor* g = call.any(args[0]);
+        if (!call.ordinary || g->dim() < 2 || g->numel() == 0 || !g->is_contiguous()) return none();
+        const int type = elem(g->scalar_type());
+        const int64_t rows = g->size(-2), cols = g->size(-1), batch = g->numel() / (rows * cols);
+        const size_t need = type < 0 || type == PPML_ELEM_I8 ? 0 : reinterpret_cast<size_t (*)(int64_t, int64_t, int64_t)>(g_launcher[NS_WS])(batch, rows, cols);
+        if (need == 0) return none();
+        Tensor out = call.empty(g->sizes(), g->scalar_type()), space = call.bytes(need);
+        const int rc = launch<cv, void*, int, int64_t, int64_t, int64_t, int, float, float, float, float, void*, size_t, void*>(
+            NS, raw(g), raw(out), type, batch, rows, cols, static_cast<int>(steps), static_cast<float>(k[0]), static_cast<float>(k[1]), static_cast<float>(k[2]),
+            static_cast<float>(k[3]), raw(space), need, nullptr);
+        return rc == 0 ? wrap(std::move(out)) : none();
+    });
+}
+
 // (name, address)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 2) { PyErr_SetString(PyExc_TypeError, "bind(name, address)"); return nullptr; }
@@ -295,6 +439,10 @@ PyMethodDef methods[] = {
     {"tri_mul_back", FAST(tri_mul_back), nullptr},
     {"flash_attn_forward", FAST(flash_attn_forward), nullptr},
     {"flash_attn_backward", FAST(flash_attn_backward), nullptr},
+    {"mul_mat_i8", FAST(mul_mat_i8), nullptr},
+    {"qk_norm_rope", FAST(qk_norm_rope), nullptr},
+    {"qk_norm_rope_backward", FAST(qk_norm_rope_backward), nullptr},
+    {"newton_schulz", FAST(newton_schulz), nullptr},
     {"bind", FAST(bind), nullptr},
     {"ready", ready, METH_O, nullptr},
     {"forget", forget, METH_NOARGS, nullptr},

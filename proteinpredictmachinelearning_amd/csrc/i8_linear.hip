@@ -613,8 +613,8 @@ extern "C" int i8_weight_pack_hip(const int8_t* w, int64_t w_stride, int M, int 
                            "i8_weight_pack_hip");
 }
 
-extern "C" size_t mul_mat_i8_workspace_hip(int N, int K) {
-    if (N <= 0 || K <= 0 || K > I8_MAX_K) return 0;
+extern "C" size_t mul_mat_i8_workspace_hip(int M, int N, int K) {
+    if (M <= 0 || M > I8_MAX_M || N <= 0 || K <= 0 || K > I8_MAX_K || i8_form(M, N, K) != I8_TILES) return 0;
     return static_cast<size_t>(N) * static_cast<size_t>(i8_row_bytes(K)) + 4 * static_cast<size_t>(N);
 }
 
@@ -626,14 +626,15 @@ extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const 
         set_error("mul_mat_i8_hip: bad arguments (M=%d N=%d K=%d x_type=%d y_type=%d)", M, N, K, x_type, y_type);
         return RC_BAD_ARGS;
     }
-    if (!workspace || workspace_bytes < mul_mat_i8_workspace_hip(N, K) || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
-        set_error("mul_mat_i8_hip: needs %zu bytes of workspace, 16-byte aligned (got %zu)", mul_mat_i8_workspace_hip(N, K), workspace_bytes);
+    const size_t need = mul_mat_i8_workspace_hip(M, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) {
+        set_error("mul_mat_i8_hip: needs %zu bytes of workspace, 16-byte aligned (got %zu)", need, workspace_bytes);
         return RC_BAD_ARGS;
     }
     StatsScope stats("i8", N, K, M, stream);
     const int64_t row = i8_row_bytes(K);
     int8_t* const q = static_cast<int8_t*>(workspace);
-    float* const scale = reinterpret_cast<float*>(q + static_cast<int64_t>(N) * row);
+    float* const scale = q ? reinterpret_cast<float*>(q + static_cast<int64_t>(N) * row) : nullptr;
     I8Product p{};
     p.w = RowBytes{reinterpret_cast<const uint8_t*>(packed), row, M};
     p.x = RowBytes{reinterpret_cast<const uint8_t*>(q), row, N};

@@ -55,11 +55,14 @@ def _not_taken(*_):
 _host = _load_host_calls()
 # each takes a call of its operator if everything about it is ordinary and answers None otherwise
 (_host_mul_mat, _host_mul_mat_f16, _host_mul_mat_q8, _host_outer_product_mean, _host_outer_prod_mean_back, _host_tri_mul, _host_tri_mul_back,
- _host_flash_attn_forward, _host_flash_attn_backward) = (
+ _host_flash_attn_forward, _host_flash_attn_backward, _host_mul_mat_i8, _host_qk_norm_rope, _host_qk_norm_rope_backward, _host_newton_schulz) = (
     getattr(_host, name, _not_taken) for name in ("mul_mat", "mul_mat_f16", "mul_mat_q8", "outer_product_mean", "outer_prod_mean_back", "tri_mul",
-                                                   "tri_mul_back", "flash_attn_forward", "flash_attn_backward"))
+                                                   "tri_mul_back", "flash_attn_forward", "flash_attn_backward", "mul_mat_i8", "qk_norm_rope",
+                                                   "qk_norm_rope_backward", "newton_schulz"))
 _HOST_LAUNCHERS = ("mul_mat_hip", "mul_mat_f16_hip", "mul_mat_q8_hip", "mul_mat_q8_ex_hip", "outer_prod_mean_hip", "outer_prod_mean_back_hip",
-                   "tri_mul_hip", "tri_mul_back_hip", "flash_attn_forward_ex_hip", "flash_attn_backward_hip")
+                   "tri_mul_hip", "tri_mul_back_hip", "flash_attn_forward_ex_hip", "flash_attn_backward_hip", "mul_mat_i8_hip",
+                   "mul_mat_i8_workspace_hip", "qk_norm_rope_hip", "qk_norm_rope_back_hip", "qk_norm_rope_back_workspace_hip", "newton_schulz_hip",
+                   "newton_schulz_workspace_hip")
 
 _initialised = set()                                  # devices ppml_hip_init has run on in this process
 
@@ -690,6 +693,11 @@ def mul_mat_i8(w: I8Weight, x, bias: torch.Tensor | None = None, dtype: torch.dt
     share one quantization.  The sums are exact.  dtype: of the result, x's by default (float32 for quantized x)."""
     if not isinstance(w, I8Weight):
         raise TypeError("mul_mat_i8: w must be an I8Weight")
+    if w._packed is not None and (dtype is None or dtype in _FLOATS):
+        q, s = x if type(x) is tuple and len(x) == 2 else (x, None)
+        y = _host_mul_mat_i8(w._packed, w.scale, w.K, q, s, bias, -1 if dtype is None else ELEM_TYPES[dtype])
+        if y is not None:
+            return y
     scale = None
     if isinstance(x, (tuple, list)):
         if len(x) != 2:
@@ -718,8 +726,8 @@ def mul_mat_i8(w: I8Weight, x, bias: torch.Tensor | None = None, dtype: torch.dt
         return out
     packed = w.pack()._packed
     x, stride = _rows(x)
-    nbytes = lib.mul_mat_i8_workspace_hip(N, K)
-    ws = _workspace(nbytes, x.device)
+    nbytes = lib.mul_mat_i8_workspace_hip(w.M, N, K)
+    ws = _workspace(nbytes, x.device) if nbytes else None
     cabi.check("mul_mat_i8_hip", lib.mul_mat_i8_hip(_ptr(packed), _ptr(w.scale), _ptr(x), ELEM_TYPES[x.dtype], stride, _ptr(scale), _ptr(bias), _ptr(out),
                                                     ELEM_TYPES[dtype], w.M, N, K, _ptr(ws), nbytes, _stream()))
     return out
@@ -789,6 +797,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None = Non
     float32, float16 or bfloat16; wq, wk float32 (d,) or None (ones).  freqs: float64 radians a position, one per pair (rope_frequencies; scaled
     ones as a long context wants them); the first 2 * len(freqs) elements of a head are turned, as pairs (i, i + len(freqs)), or of neighbours
     where `interleaved`; None turns nothing.  positions: int32 / int64 (B, L) or (L,); None: 0, 1, ..."""
+    both = _host_qk_norm_rope(q, k, wq, wk, freqs, positions, eps, interleaved)
+    if both is not None:
+        return both
     a, q, k, wq, wk, freqs, positions = _qk_norm_desc("qk_norm_rope", q, k, wq, wk, freqs, positions, eps, interleaved)
     yq, yk = (torch.empty((a.B, t.shape[2], a.L, a.d), dtype=q.dtype, device=q.device) for t in (q, k))
     a.q_out_strides, a.k_out_strides = _steps(yq, (0, 2, 1)), _steps(yk, (0, 2, 1))
@@ -804,6 +815,10 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
     """Gradients of qk_norm_rope for dq (B, hq, L, d), dk (B, hk, L, d) and its inputs: (dq (B, L, hq, d), dk (B, L, hk, d), dwq, dwk), the last two
     None without weights.  out: the fused projection's gradient, contiguous (B, L, C) with C >= (hq + hk) d: q's heads are then written
     to its first columns, k's behind them, the rest (the values') stays as it is, and the first two results are views of it."""
+    if out is None:
+        grads = _host_qk_norm_rope_backward(dq, dk, q, k, wq, wk, freqs, positions, eps, interleaved)
+        if grads is not None:
+            return grads
     a, q, k, wq, wk, freqs, positions = _qk_norm_desc("qk_norm_rope_backward", q, k, wq, wk, freqs, positions, eps, interleaved)
     dq, dk = _heads(dq, "dq", q), _heads(dk, "dk", q)
     for t, h, name in ((dq, a.hq, "dq"), (dk, a.hk, "dk")):
@@ -840,6 +855,10 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ_CO
     """An update orthogonalised by Newton-Schulz products: X = g / (|g| + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T,
     for every matrix of g [..., rows, cols] (float32, float16, bfloat16; binary32-grade arithmetic for all) -> the same shape and type.
     Singular values above a hundredth or so of the largest come out near 1.  coefficients: (a, b, c)."""
+    if type(coefficients) is tuple and len(coefficients) == 3:
+        out = _host_newton_schulz(g, steps, *coefficients, eps)
+        if out is not None:
+            return out
     g = _operand(g, "g")
     if g.dim() < 2:
         raise ValueError(f"newton_schulz: g must be a matrix or a stack of them, got {tuple(g.shape)}")

@@ -28,10 +28,10 @@ def test_quantizer_and_weight(lib):
 
 
 def test_product(lib):
-    need = lib.mul_mat_i8_workspace_hip(3, 40)
-    assert need >= 3 * 128 + 12 and lib.mul_mat_i8_workspace_hip(0, 40) == 0 and lib.mul_mat_i8_workspace_hip(3, 131072) == 0
-    ok = dict(w=ONE, ws=ONE, x=ONE, xt=0, stride=40, xs=None, bias=None, y=ONE, yt=0, M=5, N=3, K=40, wsp=ONE, nbytes=need)
-    for bad in (dict(w=None), dict(ws=None), dict(x=None), dict(y=None), dict(M=0), dict(M=(1 << 22) + 1), dict(N=0), dict(K=0), dict(K=131072, stride=131072), dict(stride=39), dict(yt=3),
+    need = lib.mul_mat_i8_workspace_hip(5, 30, 600)
+    assert need >= 30 * 640 + 120 and [lib.mul_mat_i8_workspace_hip(*s) for s in ((0, 30, 600), (5, 0, 600), (5, 30, 131072), (5, 3, 40))] == [0] * 4
+    ok = dict(w=ONE, ws=ONE, x=ONE, xt=0, stride=600, xs=None, bias=None, y=ONE, yt=0, M=5, N=30, K=600, wsp=ONE, nbytes=need)
+    for bad in (dict(w=None), dict(ws=None), dict(x=None), dict(y=None), dict(M=0), dict(M=(1 << 22) + 1), dict(N=0), dict(K=0), dict(K=131072, stride=131072), dict(stride=599), dict(yt=3),
                 dict(yt=9), dict(xt=5), dict(xt=3), dict(w=C.c_void_p(4097)), dict(wsp=None), dict(nbytes=need - 1), dict(wsp=C.c_void_p(4100))):
         a = dict(ok, **bad)
         assert lib.mul_mat_i8_hip(a["w"], a["ws"], a["x"], a["xt"], a["stride"], a["xs"], a["bias"], a["y"], a["yt"], a["M"], a["N"], a["K"], a["wsp"], a["nbytes"], None) == 1, bad
@@ -84,3 +84,12 @@ def test_operators_refuse_host_tensors():
         with pytest.raises(TypeError):
             call()
     assert torch.equal(ops.rope_frequencies(4, base=100.0, device="cpu"), torch.tensor([1.0, 0.1], dtype=torch.float64))
+
+
+def test_the_native_host_side_answers_none_to_what_is_not_ordinary():
+    x = torch.zeros(2, 3, 2, 8)
+    for name, n in (("mul_mat_i8", 7), ("qk_norm_rope", 8), ("qk_norm_rope_backward", 10), ("newton_schulz", 6)):
+        call = getattr(ops._host, name)
+        assert call() is None and call(*[None] * n) is None and call(*[x] * n) is None and call(*[1] * n) is None and call(*[None] * 12) is None
+    assert ops._host.newton_schulz(x, 5, 1.0, 1.0, 1.0, 1e-7) is None
+    assert ops._host.qk_norm_rope(x, x, None, None, None, None, 1e-6, False) is None

@@ -120,3 +120,37 @@ def test_a_step_of_training_captured(ops):
         graph.replay()
         kept = [t.clone() for t in out]
         assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+def test_the_native_host_side_gives_what_the_long_way_gives(ops, monkeypatch):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(70, 96, device="cuda", generator=gen)
+    weight = ops.I8Weight.from_f32(torch.randn(50, 96, device="cuda", generator=gen)).pack()
+    bias = torch.randn(50, device="cuda", generator=gen)
+    ready = ops.quantize_rows_i8(x)
+    qkv = torch.randn(2, 9, 4 * 16, device="cuda", generator=gen)
+    q, k = qkv[..., :32].unflatten(-1, (2, 16)), qkv[..., 32:48].unflatten(-1, (1, 16))
+    w = torch.randn(16, device="cuda", generator=gen)
+    dq, dk = torch.randn(2, 2, 9, 16, device="cuda", generator=gen), torch.randn(2, 9, 1, 16, device="cuda", generator=gen).transpose(1, 2)
+    freqs, positions = ops.rope_frequencies(8), torch.arange(9, device="cuda") * 3
+    g = torch.randn(3, 40, 30, device="cuda", generator=gen)
+    calls = [lambda: ops.mul_mat_i8(weight, x), lambda: ops.mul_mat_i8(weight, x.half(), bias, dtype=torch.bfloat16), lambda: ops.mul_mat_i8(weight, ready, bias),
+             lambda: ops.qk_norm_rope(q, k, w, None, freqs, positions, 1e-5, True), lambda: ops.qk_norm_rope(q.bfloat16(), k.bfloat16()),
+             lambda: ops.qk_norm_rope_backward(dq, dk, q, k, w, None, freqs, positions, 1e-5, True), lambda: ops.qk_norm_rope_backward(dq, dk, q, k, None, w),
+             lambda: ops.newton_schulz(g), lambda: ops.newton_schulz(g[0].half(), 3, (1.5, -0.5, 0.0), 1e-3)]
+    hosts = ("mul_mat_i8", "qk_norm_rope", "qk_norm_rope_backward", "newton_schulz")
+    taken = []
+    for name in hosts:
+        def watch(*args, _host=getattr(ops, "_host_" + name)):
+            out = _host(*args)
+            taken.append(out is not None)
+            return out
+
+        monkeypatch.setattr(ops, "_host_" + name, watch)
+    fast = [c() for c in calls]
+    assert taken == [True] * len(calls)
+    for name in hosts:
+        monkeypatch.setattr(ops, "_host_" + name, ops._not_taken)
+    for a, b in zip(fast, [c() for c in calls]):
+        for s, t in zip(*[(v if isinstance(v, tuple) else (v,)) for v in (a, b)]):
+            assert (s is None and t is None) or (s.dtype == t.dtype and torch.equal(s, t))
