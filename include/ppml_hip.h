@@ -453,8 +453,8 @@ int qk_norm_rope_back_hip(const ppml_qk_norm_desc *desc, const void *dq, const v
                           ppml_hip_stream_t stream);
 
 /* Updates orthogonalised by Newton-Schulz products: X = g / (|g| + eps), then `steps` (1 to 32) times A = X X^T, X <- a X + (b A + c A A) X, on each of
- * `batch` dense matrices of rows x cols (both up to 2^20; a matrix with more rows than columns is worked on transposed, which gives the same).  |g| is the Frobenius norm.  g and
- * out may be the same.  Binary32-grade arithmetic for every type; one rounding on the way out.  A matrix that holds an infinity or a NaN is NaN throughout.
+ * `batch` dense matrices of rows x cols (both up to 2^20; a matrix with more rows than columns is worked on transposed, which gives the same).  |g| is the Frobenius norm.  Coefficients under which
+ * singular values of up to 1 would grow beyond 2^20 are refused.  g and out may be the same.  Binary32-grade arithmetic for every type; one rounding on the way out.  A matrix that holds an infinity or a NaN is NaN throughout.
  * The workspace, newton_schulz_workspace_hip bytes, 256-byte aligned, is the call's until its work has run. */
 size_t newton_schulz_workspace_hip(int64_t batch, int64_t rows, int64_t cols);
 int newton_schulz_hip(const void *g, void *out, int type, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps,

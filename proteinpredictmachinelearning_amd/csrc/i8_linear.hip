@@ -579,7 +579,7 @@ int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* sca
     const auto tiles = [&](int side) { return static_cast<double>((p.w.rows + side - 1) / side) * static_cast<double>((p.x.rows + static_cast<int64_t>(side) - 1) / side); };
     switch (tile_side(tiles, 2.2)) {
         case 256: return launch_tiles<T, TilePingPong<StepI8>, false>(p, stream);
-        case 128: return launch_tiles<T, TileDeep<StepI8, 2, 2, 4, 4>, true>(p, stream);
+        case 128: return launch_tiles<T, TileDeep<StepI8, 2, 4, 4, 2>, true>(p, stream);
         default:  return launch_tiles<T, TileDeep<StepI8, 2, 2, 2, 2>, true>(p, stream);
     }
 }

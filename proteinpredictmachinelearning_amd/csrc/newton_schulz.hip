@@ -30,7 +30,7 @@ struct NsFactors { float of_sum[3 * NS_MOST_STEPS], of_added[3 * NS_MOST_STEPS];
 struct NsCoefficients { float a, b, c; };
 
 // the largest |p(s)| for 0 <= s <= v
-__device__ double next_bound(double v, const NsCoefficients& k) {
+__host__ __device__ double next_bound(double v, const NsCoefficients& k) {
     const auto p = [&](double s) { const double z = s * s; return fabs(s * (k.a + z * (k.b + z * k.c))); };
     double most = p(v);
     // p'(s) = a + 3 b z + 5 c z^2 = 0, z = s^2
@@ -377,6 +377,16 @@ int ns_norm_blocks(int64_t batch, int64_t count) {
     return static_cast<int>(n < 1 ? 1 : (n < NS_NORM_BLOCKS ? n : NS_NORM_BLOCKS));
 }
 
+// Whether singular values of up to 1 stay below 2^20 in every step: beyond, the bounds that the operands are scaled by say too little
+bool ns_stays(int steps, const NsCoefficients& k) {
+    double bound = 1.0;
+    for (int s = 0; s < steps; ++s) {
+        bound = next_bound(bound, k);
+        if (!(bound <= 1048576.0)) return false;
+    }
+    return true;
+}
+
 bool ns_fits(int64_t batch, int64_t rows, int64_t cols) {
     return batch > 0 && batch <= 65535 && rows > 0 && cols > 0 && rows <= NS_MOST_SIDE && cols <= NS_MOST_SIDE;
 }
@@ -418,7 +428,7 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
         };
         switch (tile_side([&](int side) { return static_cast<double>(ns_tiles(p, side)) * static_cast<double>(batch); }, 2.55)) {
             case 256: launch(TilePingPong<StepF16x2>{}, std::false_type{}); break;
-            case 128: launch(TileDeep<StepF16x2, 2, 2, 4, 4>{}, std::true_type{}); break;
+            case 128: launch(TileDeep<StepF16x2, 2, 4, 4, 2>{}, std::true_type{}); break;
             default:  launch(TileDeep<StepF16x2, 2, 2, 2, 2>{}, std::true_type{}); break;
         }
     };
@@ -471,6 +481,10 @@ extern "C" int newton_schulz_hip(const void* g, void* out, int type, int64_t bat
     const auto finite = [](float x) { return x - x == 0.0f; };
     if (!g || !out || !ns_fits(batch, rows, cols) || steps < 1 || steps > NS_MOST_STEPS || !finite(a) || !finite(b) || !finite(c) || !finite(eps) || eps < 0.0f) {
         set_error("newton_schulz_hip: bad arguments (batch=%lld rows=%lld cols=%lld steps=%d)", (long long)batch, (long long)rows, (long long)cols, steps);
+        return RC_BAD_ARGS;
+    }
+    if (!ns_stays(steps, NsCoefficients{a, b, c})) {
+        set_error("newton_schulz_hip: under coefficients %g, %g, %g singular values of up to 1 grow beyond 2^20 in %d steps", a, b, c, steps);
         return RC_BAD_ARGS;
     }
     if (!workspace || workspace_bytes < newton_schulz_workspace_hip(batch, rows, cols) || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) {

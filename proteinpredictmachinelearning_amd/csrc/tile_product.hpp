@@ -275,14 +275,19 @@ struct TilePingPong {
     }
 };
 
-// Tiles of 256 (TilePingPong), 128 or 64 (TileDeep) a side: whichever is done first.  A round of them over the CUs takes, per stage: `large`, 0.78 and
-// 0.32 us (measured: in two halves 4096 x 4096 x 4096 327 us with 256 a side and 397 with 128, 2048 x 2048 x 2048 138, 54 and 81 with 64, 1024 x 1024 x 1024
-// symmetric 24 with 128 and 12 with 64; in 8-bit integers over 4096, N tokens onto 4096 channels, quantizer included: N = 256 55, 26 and 19,
-// 1024 60, 33 and 49, 4096 85, 115 and 174).  Two work-groups of the smallest share a CU, so that a part of a round is not a whole one.
+// Tiles of 256 (TilePingPong), 128 or 64 (TileDeep) a side: whichever is done first.  A round of them over all CUs takes, per stage: `large`, 0.74 and
+// 0.32 us; a round of few takes a bit more than half of that (alone, a work-group has the caches and the power to itself), and two work-groups of the
+// smallest share a CU, so that a part of a round of those is just that part.  Measured: in two halves 4096 x 4096 x 4096 327 us with 256 a side and 397
+// with 128 (its symmetric products 247 and 209), 2048 x 2048 x 2048 138, 49 and 81 with 64, 1536 x 1536 x 1536 symmetric 33 with 128 and 23 with 64; in
+// 8-bit integers over 4096, N tokens onto 4096 channels, quantizer included: N = 256 55, 26 and 19, 1024 60, 33 and 49, 4096 85, 115 and 174.
 template <class Tiles>
 int tile_side(const Tiles& tiles, double large) {
     const double cus = device_cu_count();
-    const double t256 = large * std::ceil(tiles(256) / cus), t128 = 0.78 * std::ceil(tiles(128) / cus), t64 = 0.32 * std::fmax(1.0, tiles(64) / cus);
+    const auto time = [&](double round, double share) {
+        const double whole = std::floor(share), part = share - whole;
+        return round * (whole + (part > 0.0 ? 0.55 + 0.45 * part : 0.0));
+    };
+    const double t256 = time(large, tiles(256) / cus), t128 = time(0.74, tiles(128) / cus), t64 = 0.32 * std::fmax(1.0, tiles(64) / cus);
     return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
 }
 

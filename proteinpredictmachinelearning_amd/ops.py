@@ -854,7 +854,8 @@ NEWTON_SCHULZ_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """An update orthogonalised by Newton-Schulz products: X = g / (|g| + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T,
     for every matrix of g [..., rows, cols] (float32, float16, bfloat16; binary32-grade arithmetic for all) -> the same shape and type.
-    Singular values above a hundredth or so of the largest come out near 1.  coefficients: (a, b, c)."""
+    Singular values above a hundredth or so of the largest come out near 1.  coefficients: (a, b, c); such
+    that singular values of up to 1 stay below 2^20."""
     if type(coefficients) is tuple and len(coefficients) == 3:
         out = _host_newton_schulz(g, steps, *coefficients, eps)
         if out is not None:

@@ -72,7 +72,8 @@ def test_newton_schulz(lib):
     assert [lib.newton_schulz_workspace_hip(*s) for s in ((0, 4, 4), (65536, 4, 4), (1, 0, 4), (1, 4, 0), (1, (1 << 20) + 1, 1))] == [0] * 5
     ok = dict(g=ONE, out=ONE, type=0, batch=2, rows=30, cols=40, steps=5, a=1.0, b=1.0, c=1.0, eps=0.0, ws=ONE, nbytes=need)
     for bad in (dict(g=None), dict(out=None), dict(type=3), dict(batch=0), dict(batch=65536), dict(rows=0), dict(cols=0), dict(steps=0), dict(steps=33), dict(a=inf), dict(b=-inf),
-                dict(c=float("nan")), dict(eps=-1e-9), dict(eps=inf), dict(ws=None), dict(ws=C.c_void_p(4096 + 128)), dict(nbytes=need - 1)):
+                dict(c=float("nan")), dict(eps=-1e-9), dict(eps=inf), dict(a=30.0, b=0.0, c=0.0), dict(steps=32, a=2.0, b=0.0, c=0.0),
+                dict(a=8.2, b=-23.6, c=17.3), dict(ws=None), dict(ws=C.c_void_p(4096 + 128)), dict(nbytes=need - 1)):
         a = dict(ok, **bad)
         assert lib.newton_schulz_hip(a["g"], a["out"], a["type"], a["batch"], a["rows"], a["cols"], a["steps"], a["a"], a["b"], a["c"], a["eps"], a["ws"], a["nbytes"], None) == 1, bad
 
