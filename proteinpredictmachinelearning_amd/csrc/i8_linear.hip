@@ -36,35 +36,45 @@ __device__ __forceinline__ float largest_of(float m, float x) {
     return m + x;
 #endif
 }
-__device__ __forceinline__ float i8_scale(float largest) {
-    // (infinite or NaN: the row's results are NaN by its scale; its values are written as zeros)
-    return largest <= 3.402823466e38f ? largest * (1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
-}
-__device__ __forceinline__ float i8_value(float x, float scale) {
-    return scale > 0.0f ? fminf(fmaxf(__builtin_rintf(x / scale), -127.0f), 127.0f) : 0.0f;
-}
-__device__ __forceinline__ uint32_t pack4(const float (&q)[4]) {
-    const uint32_t a = static_cast<uint32_t>(static_cast<int>(q[0])), b = static_cast<uint32_t>(static_cast<int>(q[1]));
-    const uint32_t c = static_cast<uint32_t>(static_cast<int>(q[2])), d = static_cast<uint32_t>(static_cast<int>(q[3]));
-    return (a & 255u) | (b & 255u) << 8 | (c & 255u) << 16 | d << 24;
-}
-// Four quantized values.  The quotient's rounding is the whole number next to x times the scale's reciprocal unless that product lies
-// within 2^-14 of a half: reciprocal, product and quotient are off by less than 127 (2^-23 + 2 * 2^-24) < 2^-15 together.  A division per
-// element costs a long row more than its way from memory (8192 rows of 4096 bf16 57 us with it, 27 without); one lane in 300 takes it.
-__device__ __forceinline__ uint32_t quantize4(const float (&x)[4], float scale, float inverse) {
-    float q[4], off = 0.0f;
+// A row's scale and what its values are divided with.  The quotient is x times the scale's reciprocal (rounded correctly, once a row), which is
+// off by less than two units in the last place, with two corrections by the remainder: the first leaves less than one unit, the second is then
+// the correctly rounded quotient (Markstein's theorem), provided that no intermediate leaves the normal numbers: rows whose largest is below
+// 2^-40 are multiplied by 2^64 first, scale and all.  (A division per element cost a long row more than its way from memory, and a kernel of few
+// tokens most of its time on fetching instructions: 32 tokens x 512 -> 512 12 us.)
+struct RowScale {
+    float scale;              // as it goes out
+    float divisor, inverse, lift;
+    uint32_t keep;            // 0 where the values are zeros: the scale is 0 or NaN
+
+    __device__ __forceinline__ RowScale() : scale(0.0f), divisor(0.0f), inverse(0.0f), lift(1.0f), keep(0) {}
+    __device__ __forceinline__ explicit RowScale(float largest) {
+        // (infinite or NaN: the row's results are NaN by its scale)
+        scale = largest <= 3.402823466e38f ? largest * (1.0f / 127.0f) : __uint_as_float(0x7fc00000u);
+        lift = largest < 0x1p-40f ? 0x1p64f : 1.0f;
+        keep = scale > 0.0f ? ~0u : 0u;
+        divisor = scale * lift;
+        inverse = 1.0f / divisor;
+    }
+};
+// Four quantized values, the first in the lowest byte.  Adding 1.5 * 2^23 rounds to whole numbers, halves to even, and leaves them in the lowest bits.
+__device__ __forceinline__ uint32_t quantize4(const float (&x)[4], const RowScale& r) {
+    uint32_t q[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float t = x[e] * inverse;
-        q[e] = __builtin_rintf(t);
-        off = largest_of(off, __builtin_fabsf(t - q[e]));
+        const float y = x[e] * r.lift, rough = y * r.inverse, near = fmaf(fmaf(-rough, r.divisor, y), r.inverse, rough);
+        const float exact = fmaf(fmaf(-near, r.divisor, y), r.inverse, near);
+        // (a scale that is itself a subnormal number may be far from the 127th part)
+        q[e] = __float_as_uint(fminf(fmaxf(exact, -127.0f), 127.0f) + 12582912.0f);
     }
-    // (a scale of zero, NaN, or too small for a reciprocal: `off` is NaN)
-    if (!(off <= 0.5f - 0x1p-14f)) {
+    const uint32_t low = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u), high = __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
+    return (low | high) & r.keep;
+}
+// Four values that are whole numbers already
+__device__ __forceinline__ uint32_t pack4(const float (&x)[4]) {
+    uint32_t q[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = i8_value(x[e], scale);
-    }
-    return pack4(q);
+    for (int e = 0; e < 4; ++e) q[e] = __float_as_uint(x[e] + 12582912.0f);
+    return __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
 }
 
 // Elements k to k + 3 of a row of four or more, zeros behind its end, in two steps: the load, which is made whatever k is (the row's last four where
@@ -118,10 +128,10 @@ __device__ __forceinline__ void quantize_resident(const I8Rows& p, int64_t first
 #pragma unroll
                 for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
             largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
-            const float scale = i8_scale(largest), inverse = __builtin_amdgcn_rcpf(scale);
+            const RowScale scale(largest);
 #pragma unroll
-            for (int i = 0; i < R; ++i) put(first + g, 4 * (lane + 64 * i), quantize4(x[i], scale, inverse));
-            scale_is(first + g, scale);
+            for (int i = 0; i < R; ++i) put(first + g, 4 * (lane + 64 * i), quantize4(x[i], scale));
+            scale_is(first + g, scale.scale);
         }
     }
 }
@@ -137,7 +147,7 @@ __device__ __forceinline__ void quantize_twice(const I8Rows& p, int64_t first, i
     };
     for (int64_t r = first; r < end; ++r) {
         const T* const row = static_cast<const T*>(p.x) + r * p.stride;
-        float scale = 0.0f, inverse = 0.0f;
+        RowScale scale;
         if constexpr (sizeof(T) > 1) {
             float largest = 0.0f;
             const auto meet = [&](const float (&x)[4]) {
@@ -162,14 +172,13 @@ __device__ __forceinline__ void quantize_twice(const I8Rows& p, int64_t first, i
                 meet(x);
             }
             largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
-            scale = i8_scale(largest);
-            inverse = __builtin_amdgcn_rcpf(scale);
-            scale_is(r, scale);
+            scale = RowScale(largest);
+            scale_is(r, scale.scale);
         }
         for (int k = 4 * lane; k < (p.K + 255) / 256 * 256; k += 256) {
             float x[4];
             load(row, k, x);
-            put(r, k, sizeof(T) == 1 ? pack4(x) : quantize4(x, scale, inverse));
+            put(r, k, sizeof(T) == 1 ? pack4(x) : quantize4(x, scale));
         }
     }
 }
@@ -343,7 +352,7 @@ __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Produ
             float x[R][4], largest = 0.0f;
 #pragma unroll
             for (int i = 0; i < R; ++i) finish4<E>(raw[i], 256 * i < piece ? k0 + 256 * i : rows.K, rows.K, x[i]);
-            float scale = 0.0f, inverse = 0.0f;
+            RowScale scale;
             if constexpr (sizeof(E) > 1) {
 #pragma unroll
                 for (int i = 0; i < R; ++i)
@@ -357,14 +366,13 @@ __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Produ
                     for (int w = 0; w < share; ++w) largest = largest_of(largest, x_scale[wave - part + w]);
                     __syncthreads();
                 }
-                scale = i8_scale(largest);
-                inverse = __builtin_amdgcn_rcpf(scale);
-                if (lane == 0 && part == 0 && t < tokens) x_scale[t] = scale;
+                scale = RowScale(largest);
+                if (lane == 0 && part == 0 && t < tokens) x_scale[t] = scale.scale;
             }
             if (t < tokens) {
 #pragma unroll
                 for (int i = 0; i < R; ++i)
-                    if (256 * i < piece) put(t, k0 + 256 * i, sizeof(E) == 1 ? pack4(x[i]) : quantize4(x[i], scale, inverse));
+                    if (256 * i < piece) put(t, k0 + 256 * i, sizeof(E) == 1 ? pack4(x[i]) : quantize4(x[i], scale));
             }
         }
     };
@@ -407,16 +415,16 @@ __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Produ
 // into LDS by all its waves, and every wave multiplies them with its channels.  One launch, x read once (once per part of 64 WAVES channels).
 // A wave quantizes four rows at a time, sixteen lanes each: the search for the largest then takes four steps for four rows (a row
 // at a time by 64 lanes, six steps each, the alignment's projection was bound by it: 39 us).
-template <class T, bool VEC, int S, int WAVES>
+template <class T, bool VEC, int S, int WAVES, int TM>
 __global__ __launch_bounds__(WAVES * 64) void i8_stay_kernel(const I8Product p, const I8Rows rows) {
-    constexpr int TM = 4, TN = WAVES / 4, TOKENS = TN * 16, PITCH = TM * 16 + 4, ROW = S * TILE_K, LDS_ROW = ROW + 16;
+    constexpr int TN = WAVES / 4, TOKENS = TN * 16, PITCH = TM * 16 + 4, ROW = S * TILE_K, LDS_ROW = ROW + 16;
     constexpr int QUADS = ROW / 64;                     // of a row per lane
     __shared__ __attribute__((aligned(16))) float out_all[WAVES][16 * PITCH];
     __shared__ __attribute__((aligned(16))) uint8_t lds_q[2][TOKENS * LDS_ROW];
     __shared__ float x_scale[2][TOKENS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tokens = p.x.rows, groups = (tokens + TOKENS - 1) / TOKENS;
-    const int mw = (blockIdx.y * WAVES + wave) * 64;
+    const int mw = (blockIdx.y * WAVES + wave) * 16 * TM;
     const RowBytes W = p.w;
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(W.base), 0, static_cast<int>(W.rows * W.stride), 0x00020000);
     v4i a[S][TM][2];
@@ -451,7 +459,9 @@ __global__ __launch_bounds__(WAVES * 64) void i8_stay_kernel(const I8Product p, 
         int group = blockIdx.x, side = 0;
         request(group);
         for (; group < groups; group += gridDim.x, side ^= 1) {
-            float x[QUADS][4], scale = given, inverse = 0.0f;
+            float x[QUADS][4];
+            RowScale scale;
+            scale.scale = given;
 #pragma unroll
             for (int i = 0; i < QUADS; ++i) finish4<E>(raw[i], k0 + 64 * i, rows.K, x[i]);
             if constexpr (sizeof(E) > 1) {
@@ -460,13 +470,12 @@ __global__ __launch_bounds__(WAVES * 64) void i8_stay_kernel(const I8Product p, 
                 for (int i = 0; i < QUADS; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
-                scale = i8_scale(row16_butterfly(largest, [](float u, float v) { return largest_of(u, v); }));
-                inverse = __builtin_amdgcn_rcpf(scale);
+                scale = RowScale(row16_butterfly(largest, [](float u, float v) { return largest_of(u, v); }));
             }
 #pragma unroll
             for (int i = 0; i < QUADS; ++i)
-                *reinterpret_cast<uint32_t*>(lds_q[side] + mine * LDS_ROW + k0 + 64 * i) = sizeof(E) == 1 ? pack4(x[i]) : quantize4(x[i], scale, inverse);
-            if ((lane & 15) == 0) x_scale[side][mine] = scale;
+                *reinterpret_cast<uint32_t*>(lds_q[side] + mine * LDS_ROW + k0 + 64 * i) = sizeof(E) == 1 ? pack4(x[i]) : quantize4(x[i], scale);
+            if ((lane & 15) == 0) x_scale[side][mine] = scale.scale;
             request(group + gridDim.x);
             __syncthreads();                            // (the group before this one was read before the last one of these)
             v4i acc[TM][TN];
@@ -530,22 +539,29 @@ int launch_tiles(I8Product p, hipStream_t stream) {
     return check_launch("mul_mat_i8_hip");
 }
 
-template <class T, bool VEC, int S, int WAVES>
+template <class T, int S, int WAVES, int TM>
 void launch_stay_waves(const I8Product& p, const I8Rows& rows, hipStream_t stream) {
-    const int parts = (p.w.rows + 64 * WAVES - 1) / (64 * WAVES), groups = (p.x.rows + 4 * WAVES - 1) / (4 * WAVES);
+    constexpr int CHANNELS = 16 * TM * WAVES;
+    const bool vec = p.w.rows % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+    const int parts = (p.w.rows + CHANNELS - 1) / CHANNELS, groups = (p.x.rows + 4 * WAVES - 1) / (4 * WAVES);
     // measured, 26368 tokens of 256: onto 256 channels 256 / 512 / 768 / 1024 work-groups of four waves 15.5 / 14.5 / 15.7 / 18.9 us (eight waves
     // 16.1), onto 768 work-groups of eight waves 25.6 / 30.0 / 33.5 / 36.9 (four waves 27.3 at best, twelve 32.5)
     int wgs = (WAVES == 4 ? 2 : 1) * device_cu_count() / parts;
     if (wgs < 1) wgs = 1;
     if (wgs > groups) wgs = groups;
-    hipLaunchKernelGGL((i8_stay_kernel<T, VEC, S, WAVES>), dim3(wgs, parts), dim3(64 * WAVES), 0, stream, p, rows);
+    const dim3 grid(wgs, parts), block(64 * WAVES);
+    if (vec) hipLaunchKernelGGL((i8_stay_kernel<T, true, S, WAVES, TM>), grid, block, 0, stream, p, rows);
+    else     hipLaunchKernelGGL((i8_stay_kernel<T, false, S, WAVES, TM>), grid, block, 0, stream, p, rows);
 }
 template <class T, int S>
 void launch_stay(const I8Product& p, const I8Rows& rows, hipStream_t stream) {
-    const bool vec = p.w.rows % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
-    const int blocks = (p.w.rows + 63) / 64;
-    if (blocks <= 4) vec ? launch_stay_waves<T, true, S, 4>(p, rows, stream) : launch_stay_waves<T, false, S, 4>(p, rows, stream);
-    else             vec ? launch_stay_waves<T, true, S, 8>(p, rows, stream) : launch_stay_waves<T, false, S, 8>(p, rows, stream);
+    // What a CU gets from memory by itself is some 40 GB/s, and the L2s begin every launch empty: the weight of a product of few tokens is spread over
+    // small work-groups as long as the large ones are fewer than three quarters of the CUs (small / large, us: 32 tokens x 512 -> 512 5.3 / 12.2, 2601 x 512 ->
+    // 512 10.0 / 13.1, 2601 x 500 -> 1001 12.8 / 15.3, 5000 x 256 -> 2048 19.3 / 16.6, 26368 x 256 -> 768 39.9 / 27.8).
+    const int64_t large = static_cast<int64_t>((p.x.rows + 31) / 32) * ((p.w.rows + 511) / 512);
+    if (4 * large <= 3 * device_cu_count()) launch_stay_waves<T, S, 4, 2>(p, rows, stream);
+    else if (p.w.rows <= 256) launch_stay_waves<T, S, 4, 4>(p, rows, stream);
+    else launch_stay_waves<T, S, 8, 4>(p, rows, stream);
 }
 
 // How a product is made

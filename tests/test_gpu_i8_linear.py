@@ -132,6 +132,33 @@ def test_ties_zeros_and_small_rows(ops, dtype):
     assert (got[1] == 0.25).all()
 
 
+def test_quotients_next_to_halves(ops):
+    """Values at and next to every half of every row's scale, up to four units in the last place either way, for scales of any mantissa: the quotient's
+    own rounding decides, and it is the division's"""
+    gen = torch.Generator().manual_seed(9)
+    rows, halves = 2000, torch.arange(-126, 127) + 0.5
+    largest = (1 + torch.rand(rows, generator=gen)) * 2.0 ** torch.randint(-100, 100, (rows,), generator=gen)
+    scale = torch.from_numpy((largest.numpy() * np.float32(1 / 127)).astype(np.float32))
+    x = (scale[:, None].double() * halves[None]).float()
+    steps = torch.randint(-4, 5, x.shape, generator=gen)
+    x = torch.from_numpy((x.numpy().view(np.int32) + steps.numpy().astype(np.int32)).view(np.float32))
+    x = torch.cat((largest[:, None], x), dim=1)
+    q, s = ops.quantize_rows_i8(x.cuda())
+    want_q, want_s = rule(x)
+    assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
+
+
+@pytest.mark.parametrize("k", [40, 300, 5000])
+def test_rows_of_any_size(ops, k):
+    """Whole rows from subnormal numbers to the largest: scales without a reciprocal, scales that are subnormal"""
+    gen = torch.Generator().manual_seed(k)
+    x = torch.randn(277, k, generator=gen, dtype=torch.float64) * 2.0 ** torch.arange(-150, 127)[:, None]
+    x = x.clamp(-3.4e38, 3.4e38).float()
+    q, s = ops.quantize_rows_i8(x.cuda())
+    want_q, want_s = rule(x)
+    assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
+
+
 def test_scales_that_vanish_in_binary32(ops):
     x = torch.zeros(3, 33, device="cuda")
     x[0, 0], x[1, :3] = 1e-44, torch.tensor([1e-40, -1e-40, 3e-41])
