@@ -308,17 +308,19 @@ __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 <<
     else                    store_tokens<false>(p, ch, lds, n0 + nw, acc, x_scale + nw);
 }
 
-// Few tokens (at most 16): what counts is the weight's way from memory.  A work-group takes 16 channels, its waves every WAVES-th stage of
+// Few tokens (at most 16) of long rows: what counts is the weight's way from memory.  A work-group takes 16 channels, its waves every WAVES-th stage of
 // k, all requested before the first product.  The tokens are quantized in every work-group, into LDS, where they are few enough for that
 // to cost less than a launch of its own.
 constexpr int I8_FEW_WAVES = 8, I8_FEW_PART = 2048;     // elements of a row that a wave quantizes at most
 __host__ __device__ constexpr int few_share(int tokens) { return tokens <= 1 ? 8 : tokens <= 2 ? 4 : tokens <= 4 ? 2 : 1; }      // waves per token
 
-template <class T>
+// ROUNDS: tokens that a wave quantizes, eight or fewer tokens by shares of the waves, more by two each.  R quads of every lane hold a wave's part
+// of a token.
+template <class T, int ROUNDS, int R>
 __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Product p, const I8Rows rows) {
     constexpr int DEEP = 8, WAVES = I8_FEW_WAVES;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_q[];      // [tokens][row + 16], behind it the sums
-    __shared__ float x_scale[16];
+    __shared__ float x_scale[16], parts_largest[WAVES];
     __shared__ int sums[WAVES][16][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tokens = p.x.rows, m0 = blockIdx.x * 16, row_bytes = p.stages * TILE_K, pitch = row_bytes + 16;
@@ -335,23 +337,27 @@ __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Produ
             for (int h = 0; h < 2; ++h) a[d][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, from, stage * TILE_K + h * 64, 0));
         }
     };
-    request(wave);
     const auto put = [&](int64_t row, int k, uint32_t v) { if (k < row_bytes) *reinterpret_cast<uint32_t*>(lds_q + row * pitch + k) = v; };
-    // a token's row goes to `share` waves; R quads of every lane hold its part of at most 256 R elements
-    constexpr int R = I8_FEW_PART / 256;
-    const int share = few_share(tokens);
+    const int share = few_share(tokens), part = wave % share, piece = (row_bytes / 4 + 64 * share - 1) / (64 * share) * 256;      // elements of a wave's part
+    const int k0 = part * piece + 4 * lane;
     const auto each = [&](auto zero) {
         typedef decltype(zero) E;
-        const int part = wave % share, piece = (row_bytes / 4 + 64 * share - 1) / (64 * share) * 256;      // elements of a wave's part
-        for (int first = 0; first < tokens; first += WAVES / share) {
-            const int t = first + wave / share, k0 = part * piece + 4 * lane;
-            const E* const row = static_cast<const E*>(rows.x) + static_cast<int64_t>(t < tokens ? t : tokens - 1) * rows.stride;
-            typename Quad<E>::Raw raw[R];
+        typename Quad<E>::Raw raw[ROUNDS][R];
+        // the tokens ahead of the weight: loads come back in their order, and the weight's way is the longer one
 #pragma unroll
-            for (int i = 0; i < R; ++i) raw[i] = fetch4<E>(row, 256 * i < piece ? k0 + 256 * i : rows.K, rows.K);
+        for (int o = 0; o < ROUNDS; ++o) {
+            const int t = wave / share + o * WAVES;
+            const E* const row = static_cast<const E*>(rows.x) + static_cast<int64_t>(t < tokens ? t : tokens - 1) * rows.stride;
+#pragma unroll
+            for (int i = 0; i < R; ++i) raw[o][i] = fetch4<E>(row, 256 * i < piece ? k0 + 256 * i : rows.K, rows.K);
+        }
+        request(wave);
+#pragma unroll
+        for (int o = 0; o < ROUNDS; ++o) {
+            const int t = wave / share + o * WAVES;
             float x[R][4], largest = 0.0f;
 #pragma unroll
-            for (int i = 0; i < R; ++i) finish4<E>(raw[i], 256 * i < piece ? k0 + 256 * i : rows.K, rows.K, x[i]);
+            for (int i = 0; i < R; ++i) finish4<E>(raw[o][i], 256 * i < piece ? k0 + 256 * i : rows.K, rows.K, x[i]);
             RowScale scale;
             if constexpr (sizeof(E) > 1) {
 #pragma unroll
@@ -359,12 +365,11 @@ __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Produ
 #pragma unroll
                     for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
                 largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
-                if (share > 1) {                        // (the loop is made once)
-                    if (lane == 0) x_scale[wave] = largest;
+                if (ROUNDS == 1 && share > 1) {
+                    if (lane == 0) parts_largest[wave] = largest;
                     __syncthreads();
                     largest = 0.0f;
-                    for (int w = 0; w < share; ++w) largest = largest_of(largest, x_scale[wave - part + w]);
-                    __syncthreads();
+                    for (int w = 0; w < share; ++w) largest = largest_of(largest, parts_largest[wave - part + w]);
                 }
                 scale = RowScale(largest);
                 if (lane == 0 && part == 0 && t < tokens) x_scale[t] = scale.scale;
@@ -570,8 +575,8 @@ constexpr int I8_FEW_LDS = 40 << 10, I8_STAY_STAGES = 4;
 I8Form i8_form(int M, int N, int K) {
     const int64_t row = i8_row_bytes(K);
     if (K < 4) return I8_TILES;                         // (the rows are fetched four elements at a time)
-    if (N <= 16 && row <= I8_FEW_PART * few_share(N) && N * (row + 16) <= I8_FEW_LDS) return I8_FEW;
     if (row <= I8_STAY_STAGES * TILE_K && (M + 511) * row < 0x7fffffff) return I8_STAY;
+    if (N <= 16 && row <= I8_FEW_PART * few_share(N) && N * (row + 16) <= I8_FEW_LDS) return I8_FEW;
     return I8_TILES;
 }
 
@@ -581,7 +586,10 @@ int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* sca
     if (form == I8_FEW) {
         const dim3 grid(static_cast<unsigned>((p.w.rows + 15) / 16));
         const size_t lds = static_cast<size_t>(p.x.rows) * (row + 16);
-        hipLaunchKernelGGL((i8_few_kernel<T>), grid, dim3(I8_FEW_WAVES * 64), lds, stream, p, rows);
+        const dim3 block(I8_FEW_WAVES * 64);
+        if (p.x.rows > I8_FEW_WAVES)              hipLaunchKernelGGL((i8_few_kernel<T, 2, I8_FEW_PART / 256>), grid, block, lds, stream, p, rows);
+        else if (row > 512 * few_share(p.x.rows)) hipLaunchKernelGGL((i8_few_kernel<T, 1, I8_FEW_PART / 256>), grid, block, lds, stream, p, rows);
+        else                                      hipLaunchKernelGGL((i8_few_kernel<T, 1, 2>), grid, block, lds, stream, p, rows);
         return check_launch("mul_mat_i8_hip");
     }
     if (form == I8_STAY) {
