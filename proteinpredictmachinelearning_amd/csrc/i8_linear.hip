@@ -289,8 +289,9 @@ __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 <<
     constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN, PITCH = TM * 16 + 4;
     __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
     __shared__ float x_scale[Loop::BN];
-    const int t = xcd_contiguous_index(blockIdx.x, p.tiles_w * p.tiles_x);
-    const int m0 = (t % p.tiles_w) * Loop::BM, n0 = (t / p.tiles_w) * Loop::BN;
+    int tm, tn;
+    tile_of(xcd_contiguous_index(blockIdx.x, p.tiles_w * p.tiles_x), p.tiles_w, p.tiles_x, tm, tn);
+    const int m0 = tm * Loop::BM, n0 = tn * Loop::BN;
     for (int i = threadIdx.x; i < Loop::BN; i += Loop::THREADS) x_scale[i] = p.x_scale[n0 + i < p.x.rows ? n0 + i : p.x.rows - 1];
     v4i acc[TM][TN];
     if constexpr (DEEP) {

@@ -236,8 +236,7 @@ __device__ __forceinline__ void ns_tile_of(const NsProduct& p, int& tm, int& tn)
         while (t >= p.tiles_n - tm) { t -= p.tiles_n - tm; ++tm; }
         tn = tm + t;
     } else {
-        tm = t % p.tiles_m;
-        tn = t / p.tiles_m;
+        tile_of(t, p.tiles_m, p.tiles_n, tm, tn);
     }
 }
 

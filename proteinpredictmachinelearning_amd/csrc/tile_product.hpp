@@ -70,6 +70,17 @@ __device__ __forceinline__ void step_tiles(const v4i (&a)[TM][2], const v4i (&b)
         for (int i = 0; i < TM; ++i) Step::template step<TERM>(a[i], b[j], acc[i][j]);
     if constexpr (TERM + 1 < Step::TERMS) step_tiles<Step, TERM + 1>(a, b, acc);
 }
+// ... with between(n) after every TM of them, n = 0, 1, ...
+template <class Step, int TERM = 0, int TM, int TN, class Between>
+__device__ __forceinline__ void step_tiles_between(const v4i (&a)[TM][2], const v4i (&b)[TN][2], typename Step::Acc (&acc)[TM][TN], const Between& between) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) Step::template step<TERM>(a[i], b[j], acc[i][j]);
+        between(TERM * TN + j);
+    }
+    if constexpr (TERM + 1 < Step::TERMS) step_tiles_between<Step, TERM + 1>(a, b, acc, between);
+}
 
 // A tile of the product: WM x WN waves, each with TM x TN tiles of 16 x 16.  In lane l, register r of acc[i][j] holds the product of A's row
 // m0 + (wave's first) + 16 i + 4 (l / 16) + r and B's row n0 + (wave's first) + 16 j + l % 16.
@@ -194,17 +205,19 @@ struct TilePingPong {
         const __amdgpu_buffer_rsrc_t ra = rows_from(A, m0), rb = rows_from(B, n0);
         const int row8 = wave * 8 + (lane >> 3), piece = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
         const uint32_t from_a = static_cast<uint32_t>(row8 * A.stride) + piece * 16u, from_b = static_cast<uint32_t>(row8 * B.stride) + piece * 16u;
-        const uint32_t step_a = static_cast<uint32_t>(WAVES * 8 * A.stride), step_b = static_cast<uint32_t>(WAVES * 8 * B.stride);
+        uint32_t step_a = static_cast<uint32_t>(WAVES * 8 * A.stride), step_b = static_cast<uint32_t>(WAVES * 8 * B.stride);
+        // one of the LOADS_A + LOADS_B loads of a stage
+        const auto request_one = [&](uint8_t* to, int stage, int n) {
+            if (n < LOADS_A) load_to_lds(ra, to + (n * WAVES + wave) * 8 * TILE_K, from_a + n * step_a, stage * TILE_K);
+            else             load_to_lds(rb, to + (BM + ((n - LOADS_A) * WAVES + wave) * 8) * TILE_K, from_b + (n - LOADS_A) * step_b, stage * TILE_K);
+        };
         const auto request = [&](uint8_t* to, int stage) {
             // (the eight offsets are added up anew for every stage: kept, they are registers that the tiles need)
-            uint32_t sa = step_a, sb = step_b;
 #if defined(__HIP_DEVICE_COMPILE__)
-            asm volatile("" : "+s"(sa), "+s"(sb));
+            asm volatile("" : "+s"(step_a), "+s"(step_b));
 #endif
 #pragma unroll
-            for (int i = 0; i < LOADS_A; ++i) load_to_lds(ra, to + (i * WAVES + wave) * 8 * TILE_K, from_a + i * sa, stage * TILE_K);
-#pragma unroll
-            for (int i = 0; i < LOADS_B; ++i) load_to_lds(rb, to + (BM + (i * WAVES + wave) * 8) * TILE_K, from_b + i * sb, stage * TILE_K);
+            for (int n = 0; n < LOADS_A + LOADS_B; ++n) request_one(to, stage, n);
         };
         const int lane_at[2] = {(lane & 15) * TILE_K + (((lane >> 4) ^ ((lane & 15) >> 1)) * 16), (lane & 15) * TILE_K + (((4 + (lane >> 4)) ^ ((lane & 15) >> 1)) * 16)};
         v4i a[TM][2], b[TN][2];
@@ -227,6 +240,19 @@ struct TilePingPong {
             __builtin_amdgcn_s_setprio(0);
 #endif
         };
+        // with the next stage's loads one by one between the matrix instructions
+        const auto contract_and_request = [&](uint8_t* to, int stage) {
+#if defined(__HIP_DEVICE_COMPILE__)
+            asm volatile("" : "+s"(step_a), "+s"(step_b));
+            __builtin_amdgcn_s_setprio(1);
+            step_tiles_between<Step>(a, b, acc, [&](int n) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (n < LOADS_A + LOADS_B) request_one(to, stage, n);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            __builtin_amdgcn_s_setprio(0);
+#endif
+        };
         const auto wait_lds = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
         const auto wait_loads = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
 #pragma unroll
@@ -236,10 +262,12 @@ struct TilePingPong {
         request(even, 0);
         wait_loads();
         bare_barrier();
+        // (past the last stage that one is requested again, into an array that nobody reads any more; group 1 begins with a product of zeros:
+        // conditions around either are branches at which the registers of all tiles have to meet)
         if (wm == 0) {
             const auto stage = [&](uint8_t* here, uint8_t* next, int s) {
-                if (s + 1 < stages) request(next, s + 1);
                 read(here);
+                request(next, s + 1 < stages ? s + 1 : s);
                 wait_lds();
                 bare_barrier();
                 contract();
@@ -254,9 +282,12 @@ struct TilePingPong {
             }
             if (s < stages) stage(even, odd, s);
         } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[i][0] = a[i][1] = v4i{};
+#pragma unroll
+            for (int j = 0; j < TN; ++j) b[j][0] = b[j][1] = v4i{};
             const auto stage = [&](uint8_t* here, uint8_t* next, int s) {
-                if (s + 1 < stages) request(next, s + 1);
-                if (s > 0) contract();
+                contract_and_request(next, s + 1 < stages ? s + 1 : s);
                 bare_barrier();
                 read(here);
                 wait_lds();
@@ -274,6 +305,16 @@ struct TilePingPong {
         }
     }
 };
+
+// The t-th tile of tiles_m x tiles_n: bands of eight rows of tiles, along the columns, so that the work-groups that run at once on one XCD (a run of
+// numbers: xcd_contiguous_index) share rows and columns of both operands.
+__device__ __forceinline__ void tile_of(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+    constexpr int BAND = 8;
+    const int band = t / (BAND * tiles_n), left = tiles_m - band * BAND, rows = left < BAND ? left : BAND;
+    t -= band * BAND * tiles_n;
+    tm = band * BAND + t % rows;
+    tn = t / rows;
+}
 
 // Tiles of 256 (TilePingPong), 128 or 64 (TileDeep) a side: whichever is done first.  A round of them over all CUs takes, per stage: `large`, 0.74 and
 // 0.32 us; a round of few takes a bit more than half of that (alone, a work-group has the caches and the power to itself), and two work-groups of the
