@@ -421,7 +421,7 @@ size_t i8_weight_row_bytes_hip(int K);
 /* Rows of a weight of int8 values (M x K, w_stride bytes apart) laid out like that: M * i8_weight_row_bytes_hip(K) bytes, 16-byte aligned */
 int i8_weight_pack_hip(const int8_t *w, int64_t w_stride, int M, int K, int8_t *packed, ppml_hip_stream_t stream);
 /* y[n * M + m] = (sum_k q[n][k] w[m][k]) * x_scale[n] * w_scale[m] + (bias ? bias[m] : 0), rounded to y_type (F32, F16 or BF16).  x (N x K, x_stride elements
- * apart) is F32, F16 or BF16 and quantized by the rule above on the way (x_scale is not read), or I8 with its x_scale.  The sums are exact.  M <= 2^22.  A token
+ * apart) is F32, F16 or BF16 and quantized by the rule above on the way (x_scale is not read), or I8 with its x_scale.  The sums are exact.  M <= 2^22, N <= 2^31 - 1024.  A token
  * whose scale is NaN is NaN throughout.  The workspace, mul_mat_i8_workspace_hip(M, N, K) bytes (0: NULL will do), 16-byte aligned, is the call's until its work
  * has run. */
 size_t mul_mat_i8_workspace_hip(int M, int N, int K);
@@ -433,7 +433,8 @@ int mul_mat_i8_hip(const int8_t *packed, const float *w_scale, const void *x, in
  * or (2 i, 2 i + 1) where `interleaved` is not 0, by the token's position times freqs[i] (rot / 2 radians a position, binary64).  Positions: int32 (position_bytes 4) or int64 (8), of batch b and
  * token l at b * position_stride + l; position_bytes 0: l.  hq or hk may be 0 (its pointers are not looked at then).
  *   y = turn(x / sqrt(mean(x^2) + eps) * w)        w (d values, binary32) may be NULL: ones
- * All arithmetic is binary32, the angles' binary64; one rounding to `type` on the way out. */
+ * All arithmetic is binary32, the angles' binary64; one rounding to `type` on the way out.  What is written shares no memory with what is read.  At least 2^26 - 4 tokens (B * L)
+ * in a call, more where heads are short: beyond, it is refused. */
 typedef struct ppml_qk_norm_desc {
     int64_t B, L;
     int32_t hq, hk, d, rot;

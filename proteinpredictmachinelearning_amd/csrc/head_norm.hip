@@ -424,6 +424,10 @@ void launch_heads(const HeadNorm& p, const HeadPlan& pl, bool back, hipStream_t 
 }
 
 int run_heads(const ppml_qk_norm_desc& a, HeadNorm p, const HeadPlan& pl, bool back, hipStream_t stream, const char* what) {
+    if (pl.blocks > 0xffffffffu / 256) {                // a launch's threads along x are counted in 32 bits
+        set_error("%s: too many tokens (%lld)", what, (long long)p.tokens);
+        return RC_BAD_ARGS;
+    }
     p.group = pl.group;
     p.heads_per_part = (a.hq + a.hk + static_cast<int>(pl.parts) - 1) / static_cast<int>(pl.parts);
     switch (a.type) {

@@ -13,7 +13,8 @@
 namespace ppmlhip {
 namespace {
 
-constexpr int I8_MAX_K = 131071, I8_MAX_M = 1 << 22;
+constexpr int I8_MAX_K = 131071, I8_MAX_M = 1 << 22, I8_MAX_N = 0x7fffffff - 1023;      // (N: a tile's end stays an int)
+constexpr int64_t LAUNCH_MOST_THREADS = 0xffffffffll;   // along x
 
 // ------------------------------------------------------------------------------------------------------------ quantizer
 struct I8Rows {
@@ -525,8 +526,8 @@ void launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, fl
 }
 int launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, float* scale, hipStream_t stream, const char* what) {
     const int pieces = (p.K + 255) / 256, per_wave = p.K < 4 ? 1 : pieces <= 1 ? 8 : pieces <= 2 ? 4 : pieces <= 4 ? 2 : 1;
+    if (p.rows > LAUNCH_MOST_THREADS / 256 * 4 * per_wave) { set_error("%s: too many rows (%lld)", what, (long long)p.rows); return RC_BAD_ARGS; }
     const int64_t waves = (p.rows + per_wave - 1) / per_wave;
-    if (waves > 4ll * 0x7fffffff) { set_error("%s: too many rows", what); return RC_BAD_ARGS; }
     switch (p.type) {
         case PPML_ELEM_F32:  launch_quantize<float>(p, q, q_stride, q_end, scale, waves, stream); break;
         case PPML_ELEM_F16:  launch_quantize<_Float16>(p, q, q_stride, q_end, scale, waves, stream); break;
@@ -540,7 +541,7 @@ template <class T, class Loop, bool DEEP>
 int launch_tiles(I8Product p, hipStream_t stream) {
     p.tiles_w = (p.w.rows + Loop::BM - 1) / Loop::BM;
     p.tiles_x = (p.x.rows + Loop::BN - 1) / Loop::BN;
-    if (static_cast<int64_t>(p.tiles_w) * p.tiles_x > 0x7fffffff) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
+    if (static_cast<int64_t>(p.tiles_w) * p.tiles_x > LAUNCH_MOST_THREADS / Loop::THREADS) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
     hipLaunchKernelGGL((i8_product_kernel<T, Loop, DEEP>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x)), dim3(Loop::THREADS), 0, stream, p);
     return check_launch("mul_mat_i8_hip");
 }
@@ -639,14 +640,14 @@ extern "C" int i8_weight_pack_hip(const int8_t* w, int64_t w_stride, int M, int 
 }
 
 extern "C" size_t mul_mat_i8_workspace_hip(int M, int N, int K) {
-    if (M <= 0 || M > I8_MAX_M || N <= 0 || K <= 0 || K > I8_MAX_K || i8_form(M, N, K) != I8_TILES) return 0;
+    if (M <= 0 || M > I8_MAX_M || N <= 0 || N > I8_MAX_N || K <= 0 || K > I8_MAX_K || i8_form(M, N, K) != I8_TILES) return 0;
     return static_cast<size_t>(N) * static_cast<size_t>(i8_row_bytes(K)) + 4 * static_cast<size_t>(N);
 }
 
 extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const void* x, int x_type, int64_t x_stride, const float* x_scale, const float* bias,
                               void* y, int y_type, int M, int N, int K, void* workspace, size_t workspace_bytes, ppml_hip_stream_t stream_) {
     const hipStream_t stream = static_cast<hipStream_t>(stream_);
-    if (!packed || !w_scale || !x || !y || M <= 0 || M > I8_MAX_M || N <= 0 || K <= 0 || K > I8_MAX_K || x_stride < K || !float_type(y_type) ||
+    if (!packed || !w_scale || !x || !y || M <= 0 || M > I8_MAX_M || N <= 0 || N > I8_MAX_N || K <= 0 || K > I8_MAX_K || x_stride < K || !float_type(y_type) ||
         (x_type == PPML_ELEM_I8 ? !x_scale : !float_type(x_type)) || (reinterpret_cast<uintptr_t>(packed) & 15) != 0) {
         set_error("mul_mat_i8_hip: bad arguments (M=%d N=%d K=%d x_type=%d y_type=%d)", M, N, K, x_type, y_type);
         return RC_BAD_ARGS;

@@ -662,8 +662,8 @@ class I8Weight:
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor):
         data, scale = _operand(data, "data", (torch.int8,)), _operand(scale, "scale", (torch.float32,))
-        if data.dim() != 2 or not 1 <= data.shape[1] <= 131071 or data.shape[0] < 1 or tuple(scale.shape) != (data.shape[0],):
-            raise ValueError(f"I8Weight: data must be [M, K] with K of 1 to 131071 and scale [M], got {tuple(data.shape)} and {tuple(scale.shape)}")
+        if data.dim() != 2 or not 1 <= data.shape[1] <= 131071 or not 1 <= data.shape[0] <= 1 << 22 or tuple(scale.shape) != (data.shape[0],):
+            raise ValueError(f"I8Weight: data must be [M, K] with M of 1 to 2^22, K of 1 to 131071 and scale [M], got {tuple(data.shape)} and {tuple(scale.shape)}")
         self.data, self.scale = data, scale.contiguous()
         self.M, self.K = data.shape
         self._packed = data if data.is_contiguous() and self.K % 128 == 0 and data.data_ptr() % 16 == 0 else None
@@ -720,6 +720,8 @@ def mul_mat_i8(w: I8Weight, x, bias: torch.Tensor | None = None, dtype: torch.dt
         if tuple(bias.shape) != (w.M,):
             raise ValueError(f"mul_mat_i8: bias {tuple(bias.shape)}, expected ({w.M},)")
     N, K = x.shape
+    if N >= (1 << 31) - 1023:
+        raise ValueError(f"mul_mat_i8: at most 2^31 - 1024 tokens a call, got {N}")
     out = torch.empty((N, w.M), dtype=dtype, device=x.device)
     lib = _lib()
     if N == 0:
@@ -761,8 +763,8 @@ def _qk_norm_desc(who, q, k, wq, wk, freqs, positions, eps, interleaved):
         raise ValueError(f"{who}: q (B, L, hq, d) {tuple(q.shape)} and k (B, L, hk, d) {tuple(k.shape)} differ in B, L or d")
     if not 1 <= d <= 512:
         raise ValueError(f"{who}: heads of 1 to 512 elements, got {d}")
-    if hq < 1 or k.shape[2] < 1:
-        raise ValueError(f"{who}: q and k need a head each")
+    if not (1 <= hq <= 65535 and 1 <= k.shape[2] <= 65535):
+        raise ValueError(f"{who}: q and k need a head each, and have 65535 at most")
     if not eps >= 0.0:
         raise ValueError(f"{who}: eps must not be negative")
     weights = []

@@ -94,3 +94,19 @@ def test_the_native_host_side_answers_none_to_what_is_not_ordinary():
         assert call() is None and call(*[None] * n) is None and call(*[x] * n) is None and call(*[1] * n) is None and call(*[None] * 12) is None
     assert ops._host.newton_schulz(x, 5, 1.0, 1.0, 1.0, 1e-7) is None
     assert ops._host.qk_norm_rope(x, x, None, None, None, None, 1e-6, False) is None
+
+
+def test_counts_past_what_a_launch_can_number(lib):
+    """Refused, neither wrapped nor left to the launch: threads along x are counted in 32 bits, tokens of a product in an int."""
+    most = 0x7fffffff - 1023
+    assert lib.mul_mat_i8_workspace_hip(5, most + 1, 600) == 0 and lib.mul_mat_i8_workspace_hip(5, most, 600) > most * 640
+    for n in (most + 1, 0x7fffffff):
+        for k in (4, 600):
+            assert lib.mul_mat_i8_hip(ONE, ONE, ONE, 0, k, None, None, ONE, 0, 5, n, k, ONE, 1 << 62, None) == 1
+            assert b"bad arguments" in lib.ppml_hip_last_error()
+    for rows, k in ((1 << 62, 1), (1 << 27, 2048), (1 << 30, 4)):
+        assert lib.quantize_rows_i8_hip(ONE, 0, k, ONE, k, ONE, rows, k, None) == 1
+        assert b"too many rows" in lib.ppml_hip_last_error()
+    for kw in (dict(B=1, L=1 << 27, hq=1, hk=0, d=512, rot=0), dict(B=1 << 16, L=1 << 16, hq=1, hk=1, d=2, rot=2)):
+        assert lib.qk_norm_rope_hip(C.byref(desc(**kw)), *[ONE] * 8, None) == 1
+        assert b"too many tokens" in lib.ppml_hip_last_error()

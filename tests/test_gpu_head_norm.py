@@ -301,3 +301,11 @@ def test_refusals(ops):
                 lambda: ops.qk_norm_rope_backward(dq, dk, q, k, out=torch.zeros(2, 3, 32, device="cuda").half())):
         with pytest.raises(TypeError):
             bad()
+
+
+def test_more_heads_than_a_launch_can_number_are_refused(ops):
+    q = torch.zeros(1, 1, 1, 4, device="cuda")
+    for h in (65536, (1 << 32) + 1):
+        for a, b in ((q.expand(1, 1, h, 4), q), (q, q.expand(1, 1, h, 4))):
+            with pytest.raises(ValueError):
+                ops.qk_norm_rope(a, b)

@@ -262,3 +262,15 @@ def test_refusals(ops):
                 lambda: ops.mul_mat_i8(W, x, torch.zeros(4, device="cuda").half()), lambda: ops.mul_mat_i8(W, w), lambda: ops.quantize_rows_i8(w)):
         with pytest.raises(TypeError):
             bad()
+
+
+def test_counts_that_an_int_cannot_hold_are_refused(ops):
+    """(rows that share memory: nothing is allocated)"""
+    w, x = torch.zeros(1, 8, dtype=torch.int8, device="cuda"), torch.zeros(1, 8, device="cuda")
+    for M in ((1 << 22) + 1, (1 << 32) + 1):
+        with pytest.raises(ValueError):
+            ops.I8Weight(w.expand(M, 8), x[0, :1].expand(M))
+    W = ops.I8Weight(w, x[0, :1])
+    for N in ((1 << 31) - 1023, (1 << 32) + 1):
+        with pytest.raises(ValueError):
+            ops.mul_mat_i8(W, x.expand(N, 8))
