@@ -16,6 +16,7 @@
 #include "elements.hpp"
 #include "tile_product.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace ppmlhip {
@@ -226,10 +227,12 @@ struct NsProduct {
     const NsFactors* factors;
     int which;                // 3 step + product
     int tiles_m, tiles_n, stages, symmetric, final_turned, final_vec;
+    // the tiles of all matrices from `whole` on are cut into slices of slice_stages stages, whose sums go to `sums` (slices = 1: none)
+    int tiles, whole, slices, slice_stages;
+    v4f* sums;                // [tile - whole][slice][a wave's tiles of 16 x 16][thread]
 };
 
-__device__ __forceinline__ void ns_tile_of(const NsProduct& p, int& tm, int& tn) {
-    int t = xcd_contiguous_index(blockIdx.x, gridDim.x);
+__device__ __forceinline__ void ns_tile_of(const NsProduct& p, int t, int& tm, int& tn) {
     if (p.symmetric) {
         // the t-th tile on or above the diagonal, by rows
         tm = 0;
@@ -302,19 +305,39 @@ template <class T, class Loop, bool DEEP>
 __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 << 10 ? Loop::WAVES / 4 : 2) void ns_product_kernel(const NsProduct p) {
     constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN;
     __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
-    const int64_t z = blockIdx.y;
+    int t = xcd_contiguous_index(blockIdx.x, p.whole), slice = -1, stages = p.stages;
+    if (DEEP && static_cast<int>(blockIdx.x) >= p.whole) {
+        const int i = blockIdx.x - p.whole;             // (slices of the same k on one XCD: they share rows of either operand)
+        slice = i % p.slices;
+        t = p.whole + i / p.slices;
+    }
+    const int64_t z = t / p.tiles;
     int tm, tn;
-    ns_tile_of(p, tm, tn);
+    ns_tile_of(p, t % p.tiles, tm, tn);
     const int m0 = tm * Loop::BM, n0 = tn * Loop::BN;
     RowBytes A = p.a, B = p.b;
     A.base += z * p.a_matrix;
     B.base += z * p.b_matrix;
+    if (DEEP && slice >= 0) {
+        const int first = slice * p.slice_stages;
+        A.base += first * TILE_K;
+        B.base += first * TILE_K;
+        stages = stages - first < p.slice_stages ? stages - first : p.slice_stages;
+    }
     v4f acc[TM][TN];
     if constexpr (DEEP) {
         __shared__ __attribute__((aligned(128))) uint8_t third[Loop::STAGE], fourth[Loop::STAGE];
-        Loop::run(A, B, m0, n0, p.stages, even, odd, third, fourth, acc);
+        Loop::run(A, B, m0, n0, stages, even, odd, third, fourth, acc);
+        if (slice >= 0) {
+            v4f* const to = p.sums + (static_cast<int64_t>(t - p.whole) * p.slices + slice) * (TM * TN * Loop::THREADS) + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) to[(i * TN + j) * Loop::THREADS] = acc[i][j];
+            return;
+        }
     } else {
-        Loop::run(A, B, m0, n0, p.stages, even, odd, acc);
+        Loop::run(A, B, m0, n0, stages, even, odd, acc);
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float of_sum = p.factors[z].of_sum[p.which], of_added = p.factors[z].of_added[p.which];
@@ -341,11 +364,59 @@ __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 <<
         }
 }
 
+// The tiles that were cut: a wave per block of 32 x 32, its slices' sums added in their order, then as above
+template <class T, class Loop>
+__global__ __launch_bounds__(64) void ns_join_kernel(const NsProduct p) {
+    constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN, BLOCKS = TM / 2 * (TN / 2), SUMS = TM * TN * Loop::THREADS;
+    __shared__ float lds[32 * NS_PITCH];
+    const int lane = threadIdx.x, wave = blockIdx.x % Loop::WAVES, block = blockIdx.x / Loop::WAVES % BLOCKS, cut = blockIdx.x / (Loop::WAVES * BLOCKS);
+    const int t = p.whole + cut, i = block / (TN / 2) * 2, j = block % (TN / 2) * 2;
+    const int64_t z = t / p.tiles;
+    int tm, tn;
+    ns_tile_of(p, t % p.tiles, tm, tn);
+    const int mb = tm * Loop::BM + (wave / WN * TM + i) * 16, nb = tn * Loop::BN + (wave % WN * TN + j) * 16;
+    Operand16 added{};
+    ns_fetch_added(p, added, z, mb, nb);
+    const v4f* const from = p.sums + static_cast<int64_t>(cut) * p.slices * SUMS + wave * 64 + lane;
+    v4f sum[4] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.slices; ++s)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[q] += from[static_cast<int64_t>(s) * SUMS + ((i + (q >> 1)) * TN + j + (q & 1)) * Loop::THREADS];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds[(16 * (q >> 1) + (lane >> 4) * 4 + r) * NS_PITCH + 16 * (q & 1) + (lane & 15)] = sum[q][r];
+    wave_fence();
+    ns_finish_block<T>(p, lds, z, mb, nb, p.symmetric && tm != tn, p.factors[z].of_sum[p.which], p.factors[z].of_added[p.which], added);
+}
+
 // ------------------------------------------------------------------------------------------------------------ host side
+typedef TilePingPong<StepF16x2> NsLarge;
+typedef TileDeep<StepF16x2, 2, 4, 4, 2> NsMiddle;
+typedef TileDeep<StepF16x2, 2, 2, 2, 2> NsSmall;
+
+// How a product of every matrix of the batch is made: tiles of `side`, the middle ones perhaps cut
+struct NsPlan { int side, tiles; CutTiles cut; };
+NsPlan ns_plan(int64_t batch, int64_t rows_a, int64_t rows_b, bool symmetric, int64_t row_bytes) {
+    const auto tiles = [&](int side) {
+        const int64_t m = (rows_a + side - 1) / side, n = (rows_b + side - 1) / side;
+        return symmetric ? n * (n + 1) / 2 : m * n;
+    };
+    const int stages = static_cast<int>(row_bytes / TILE_K);
+    const CutTiles cut = cut_tiles(batch * tiles(128), stages);
+    NsPlan plan{};
+    plan.side = tile_side([&](int side) { return static_cast<double>(batch * tiles(side)); }, 2.55, cut.rounds);
+    plan.tiles = static_cast<int>(tiles(plan.side));
+    plan.cut = plan.side == 128 ? cut : CutTiles{batch * plan.tiles, 0, 1, stages, 0.0};
+    return plan;
+}
+
 struct NsLayout {
     int64_t m, n;             // m <= n
     int64_t x_stride, xt_stride, sq_stride;              // bytes of a row of X, of X^T and A
-    int64_t x, xt, x2, xt2, a, b, partial, factors, total;
+    int64_t x, xt, x2, xt2, a, b, partial, factors, sums, total;
+    NsPlan gram, poly, next;
 };
 int64_t operand_row(int64_t k) { return (k + 31) / 32 * 128; }
 
@@ -365,6 +436,12 @@ NsLayout ns_layout(int64_t batch, int64_t rows, int64_t cols) {
     l.b = take(batch * l.m * l.sq_stride);
     l.partial = take(batch * NS_NORM_BLOCKS * 8);
     l.factors = take(batch * static_cast<int64_t>(sizeof(NsFactors)));
+    l.gram = ns_plan(batch, l.m, l.m, true, l.x_stride);
+    l.poly = ns_plan(batch, l.m, l.m, true, l.sq_stride);
+    l.next = ns_plan(batch, l.m, l.n, false, l.sq_stride);
+    int64_t most = 0;
+    for (const NsPlan* plan : {&l.gram, &l.poly, &l.next}) most = std::max(most, plan->cut.left * plan->cut.slices);
+    l.sums = take(most * NsMiddle::BM * NsMiddle::BN * 4);
     l.total = at;
     return l;
 }
@@ -390,11 +467,6 @@ bool ns_fits(int64_t batch, int64_t rows, int64_t cols) {
     return batch > 0 && batch <= 65535 && rows > 0 && cols > 0 && rows <= NS_MOST_SIDE && cols <= NS_MOST_SIDE;
 }
 
-int64_t ns_tiles(const NsProduct& p, int side) {
-    const int64_t m = (p.a.rows + side - 1) / side, n = (p.b.rows + side - 1) / side;
-    return p.symmetric ? n * (n + 1) / 2 : m * n;
-}
-
 template <class T>
 int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int64_t cols, int steps, const NsCoefficients& k, float eps, uint8_t* ws,
                       hipStream_t stream) {
@@ -415,21 +487,29 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
                        0, stream, s);
     uint8_t *x = ws + l.x, *xt = ws + l.xt, *x2 = ws + l.x2, *xt2 = ws + l.xt2;
     const int64_t sq_matrix = l.m * l.sq_stride;
-    const auto product = [&](NsProduct p) {
+    const auto product = [&](NsProduct p, const NsPlan& plan) {
         p.factors = factors;
         p.final_vec = out_vec;
+        p.tiles = plan.tiles;
+        p.whole = static_cast<int>(plan.cut.whole);
+        p.slices = plan.cut.slices;
+        p.slice_stages = plan.cut.stages;
+        p.sums = reinterpret_cast<v4f*>(ws + l.sums);
         const auto launch = [&](auto loop, auto deep) {
             typedef decltype(loop) Loop;
             p.tiles_m = (p.a.rows + Loop::BM - 1) / Loop::BM;
             p.tiles_n = (p.b.rows + Loop::BN - 1) / Loop::BN;
-            hipLaunchKernelGGL((ns_product_kernel<T, Loop, decltype(deep)::value>), dim3(static_cast<unsigned>(ns_tiles(p, Loop::BM)), static_cast<unsigned>(batch)),
+            hipLaunchKernelGGL((ns_product_kernel<T, Loop, decltype(deep)::value>), dim3(static_cast<unsigned>(plan.cut.whole + plan.cut.left * plan.cut.slices)),
                                dim3(Loop::THREADS), 0, stream, p);
         };
-        switch (tile_side([&](int side) { return static_cast<double>(ns_tiles(p, side)) * static_cast<double>(batch); }, 2.55)) {
-            case 256: launch(TilePingPong<StepF16x2>{}, std::false_type{}); break;
-            case 128: launch(TileDeep<StepF16x2, 2, 4, 4, 2>{}, std::true_type{}); break;
-            default:  launch(TileDeep<StepF16x2, 2, 2, 2, 2>{}, std::true_type{}); break;
+        switch (plan.side) {
+            case 256: launch(NsLarge{}, std::false_type{}); break;
+            case 128: launch(NsMiddle{}, std::true_type{}); break;
+            default:  launch(NsSmall{}, std::true_type{}); break;
         }
+        if (plan.cut.left > 0)
+            hipLaunchKernelGGL((ns_join_kernel<T, NsMiddle>), dim3(static_cast<unsigned>(plan.cut.left * NsMiddle::WAVES * (NsMiddle::TM / 2) * (NsMiddle::TN / 2))), dim3(64), 0,
+                               stream, p);
     };
     const int m = static_cast<int>(l.m), n = static_cast<int>(l.n);
     for (int step = 0; step < steps; ++step) {
@@ -438,14 +518,14 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
         gram.a_matrix = gram.b_matrix = l.m * l.x_stride;
         gram.out = ws + l.a; gram.out_matrix = sq_matrix; gram.out_stride = l.sq_stride;
         gram.which = 3 * step; gram.symmetric = 1; gram.stages = static_cast<int>(l.x_stride / TILE_K);
-        product(gram);
+        product(gram, l.gram);
         NsProduct poly{};
         poly.a = poly.b = RowBytes{ws + l.a, l.sq_stride, m};
         poly.a_matrix = poly.b_matrix = sq_matrix;
         poly.added = ws + l.a; poly.added_matrix = sq_matrix; poly.added_stride = l.sq_stride;
         poly.out = ws + l.b; poly.out_matrix = sq_matrix; poly.out_stride = l.sq_stride;
         poly.which = 3 * step + 1; poly.symmetric = 1; poly.stages = static_cast<int>(l.sq_stride / TILE_K);
-        product(poly);
+        product(poly, l.poly);
         NsProduct next{};
         next.a = RowBytes{ws + l.b, l.sq_stride, m};
         next.b = RowBytes{xt, l.xt_stride, n};
@@ -458,7 +538,7 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
         } else {
             next.final = out; next.final_matrix = count; next.final_turned = rows > cols;
         }
-        product(next);
+        product(next, l.next);
         uint8_t* const keep = x; x = x2; x2 = keep;
         uint8_t* const keep_t = xt; xt = xt2; xt2 = keep_t;
     }

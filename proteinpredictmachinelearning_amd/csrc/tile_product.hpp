@@ -321,15 +321,36 @@ __device__ __forceinline__ void tile_of(int t, int tiles_m, int tiles_n, int& tm
 // smallest share a CU, so that a part of a round of those is just that part.  Measured: in two halves 4096 x 4096 x 4096 327 us with 256 a side and 397
 // with 128 (its symmetric products 247 and 209), 2048 x 2048 x 2048 138, 49 and 81 with 64, 1536 x 1536 x 1536 symmetric 33 with 128 and 23 with 64; in
 // 8-bit integers over 4096, N tokens onto 4096 channels, quantizer included: N = 256 55, 26 and 19, 1024 60, 33 and 49, 4096 85, 115 and 174.
+// `cut`: what the last, partial round of tiles of 128 takes instead where its tiles are cut along k (CutTiles), in rounds; 0: they are not.
+inline double partial_round(double part) { return part > 0.0 ? 0.55 + 0.45 * part : 0.0; }
 template <class Tiles>
-int tile_side(const Tiles& tiles, double large) {
+int tile_side(const Tiles& tiles, double large, double cut = 0.0) {
     const double cus = device_cu_count();
-    const auto time = [&](double round, double share) {
+    const auto time = [&](double round, double share, double last) {
         const double whole = std::floor(share), part = share - whole;
-        return round * (whole + (part > 0.0 ? 0.55 + 0.45 * part : 0.0));
+        return round * (whole + (last > 0.0 ? last : partial_round(part)));
     };
-    const double t256 = time(large, tiles(256) / cus), t128 = time(0.74, tiles(128) / cus), t64 = 0.32 * std::fmax(1.0, tiles(64) / cus);
+    const double t256 = time(large, tiles(256) / cus, 0.0), t128 = time(0.74, tiles(128) / cus, cut), t64 = 0.32 * std::fmax(1.0, tiles(64) / cus);
     return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+}
+
+// The tiles of 128 behind the last whole round, each cut along k into `slices` work-groups of `stages` stages (the last of them perhaps fewer), so that
+// together they fill the CUs once; their sums are joined by a launch of its own, in their order.  slices = 1: not worth that launch and its way
+// through memory, 10 us.  Measured, five steps of newton_schulz.hip without / with: 4096 x 4096 (528 tiles of a symmetric product) 3938 / 3465 us,
+// 2944 x 2944 (276) 1963 / 1542; 3968 x 4096 (496: none are cut) 3345 / 3217 from tiles numbered through all matrices alone.
+struct CutTiles { int64_t whole, left; int slices, stages; double rounds; };
+inline CutTiles cut_tiles(int64_t tiles, int stages) {
+    const int64_t cus = device_cu_count();
+    CutTiles c{tiles, 0, 1, stages, 0.0};
+    const int64_t left = tiles % cus;
+    if (tiles < cus || left == 0) return c;
+    int64_t slices = cus / left < stages / 4 ? cus / left : stages / 4;
+    if (slices < 2) return c;
+    const int each = static_cast<int>((stages + slices - 1) / slices);
+    slices = (stages + each - 1) / each;
+    const double rounds = (each + 10.0 / 0.74) / stages;
+    if (rounds < partial_round(static_cast<double>(left) / static_cast<double>(cus))) c = CutTiles{tiles - left, left, static_cast<int>(slices), each, rounds};
+    return c;
 }
 
 }  // namespace

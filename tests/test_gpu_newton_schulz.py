@@ -74,6 +74,16 @@ def test_large_stacks(ops, shape):
         check(ops.newton_schulz(g, steps=steps), g, steps)
 
 
+# a little more than a whole round of tiles of 128 over 256 CUs: the rest is cut along the long axis (A alone; B X alone, either way round; all three)
+@pytest.mark.parametrize("shape,dtype", [((28, 500, 1001), torch.float32), ((28, 1024, 512), torch.bfloat16), ((4, 1000, 1050), torch.float16), ((4, 1050, 1000), torch.float32),
+                                         ((8, 900, 1000), torch.float32)])
+def test_tiles_behind_a_whole_round(ops, shape, dtype):
+    g = update(shape, dtype, seed=12)
+    first = ops.newton_schulz(g, steps=2)
+    check(first, g, 2)
+    assert torch.equal(ops.newton_schulz(g, steps=2), first)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(24, 72), (3, 100, 64), (160, 160)])
 def test_types(ops, shape, dtype):
