@@ -186,6 +186,11 @@ __device__ __forceinline__ float squares_of(const float (&a)[R][V], const float 
     return sum;
 }
 
+// Forward.  Bound by memory, a head read and written once: all of a token's heads pass through one group of lanes, so that the angles (64-bit work, as much as
+// several heads') are made once, and the next head is on its way while one is normed.  Few tokens: the heads are cut into parts too (plan_heads),
+// which make their angles again.  Measured: 26368 tokens of 16 heads of 32, f32 26.6 us (4.1 TB/s, where a large copy reaches 5.2; 19.0 where the last-level
+// cache holds the tensors); 32768 of 40 heads of 128, bf16 155 us (4.3 TB/s); 103 tokens of 16 heads 4.2 us, an empty launch and one way to memory.
+// Non-temporal loads and stores: the same or slower.
 template <class T, int V, int R, bool INTER, bool FULL>
 __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNorm p) {
     const int lane = threadIdx.x & (p.group - 1);
@@ -234,6 +239,10 @@ __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNorm p) {
     }
 }
 
+// Backward, the norm's statistics made again (reading them back would cost as much as the rows they are of): x and dy in, dx out, one pass, bound by
+// memory.  The weights' gradients stay in the lanes over all of a work-group's tokens and leave as one partial sum per work-group, in a fixed order: no
+// atomics, the same bits every time.  Measured: 26368 tokens of 16 heads of 32, f32 42.8 us (3.8 TB/s; 34 where the last-level cache holds the tensors), of which
+// 4.7 are the launch that adds the partial sums.
 template <class T, int V, int R, bool INTER, bool FULL>
 __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
     extern __shared__ __attribute__((aligned(16))) float lds[];      // [tokens of the work-group][d]
