@@ -404,7 +404,7 @@ typedef TilePingPong<StepF16x2> NsLarge;
 typedef TileDeep<StepF16x2, 2, 4, 4, 2> NsMiddle;
 typedef TileDeep<StepF16x2, 2, 2, 2, 2> NsSmall;
 
-// How a product of every matrix of the batch is made: tiles of `side`, the middle ones perhaps cut
+// How a product of every matrix of the batch is made: tiles of `side`, the middle and small ones perhaps cut
 struct NsPlan { int side, tiles; CutTiles cut; };
 NsPlan ns_plan(int64_t batch, int64_t rows_a, int64_t rows_b, bool symmetric, int64_t row_bytes) {
     const auto tiles = [&](int side) {
@@ -412,11 +412,11 @@ NsPlan ns_plan(int64_t batch, int64_t rows_a, int64_t rows_b, bool symmetric, in
         return symmetric ? n * (n + 1) / 2 : m * n;
     };
     const int stages = static_cast<int>(row_bytes / TILE_K);
-    const CutTiles cut = cut_tiles(batch * tiles(128), stages);
+    const CutTiles cut = cut_tiles(batch * tiles(128), stages), few = cut_few_tiles(batch * tiles(64), stages, 0.2);
     NsPlan plan{};
-    plan.side = tile_side([&](int side) { return static_cast<double>(batch * tiles(side)); }, 2.55, cut.rounds);
+    plan.side = tile_side([&](int side) { return static_cast<double>(batch * tiles(side)); }, 2.55, cut.rounds, few.rounds);
     plan.tiles = static_cast<int>(tiles(plan.side));
-    plan.cut = plan.side == 128 ? cut : CutTiles{batch * plan.tiles, 0, 1, stages, 0.0};
+    plan.cut = plan.side == 128 ? cut : plan.side == 64 ? few : CutTiles{batch * plan.tiles, 0, 1, stages, 0.0};
     return plan;
 }
 
@@ -448,8 +448,8 @@ NsLayout ns_layout(int64_t batch, int64_t rows, int64_t cols) {
     l.poly = ns_plan(batch, l.m, l.m, true, l.sq_stride);
     l.next = ns_plan(batch, l.m, l.n, false, l.sq_stride);
     int64_t most = 0;
-    for (const NsPlan* plan : {&l.gram, &l.poly, &l.next}) most = std::max(most, plan->cut.left * plan->cut.slices);
-    l.sums = take(most * NsMiddle::BM * NsMiddle::BN * 4);
+    for (const NsPlan* plan : {&l.gram, &l.poly, &l.next}) most = std::max(most, plan->cut.left * plan->cut.slices * plan->side * plan->side * 4);
+    l.sums = take(most);
     l.total = at;
     return l;
 }
@@ -515,9 +515,14 @@ int run_newton_schulz(const void* g, void* out, int64_t batch, int64_t rows, int
             case 128: launch(NsMiddle{}, std::true_type{}); break;
             default:  launch(NsSmall{}, std::true_type{}); break;
         }
-        if (plan.cut.left > 0)
-            hipLaunchKernelGGL((ns_join_kernel<T, NsMiddle>), dim3(static_cast<unsigned>(plan.cut.left * NsMiddle::WAVES * (NsMiddle::TM / 2) * (NsMiddle::TN / 2))), dim3(64), 0,
-                               stream, p);
+        const auto join = [&](auto loop) {
+            typedef decltype(loop) Loop;
+            hipLaunchKernelGGL((ns_join_kernel<T, Loop>), dim3(static_cast<unsigned>(plan.cut.left * Loop::WAVES * (Loop::TM / 2) * (Loop::TN / 2))), dim3(64), 0, stream, p);
+        };
+        if (plan.cut.left > 0) {
+            if (plan.side == 128) join(NsMiddle{});
+            else join(NsSmall{});
+        }
     };
     const int m = static_cast<int>(l.m), n = static_cast<int>(l.n);
     for (int step = 0; step < steps; ++step) {

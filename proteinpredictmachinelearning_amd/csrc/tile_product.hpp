@@ -321,16 +321,17 @@ __device__ __forceinline__ void tile_of(int t, int tiles_m, int tiles_n, int& tm
 // smallest share a CU, so that a part of a round of those is just that part.  Measured: in two halves 4096 x 4096 x 4096 327 us with 256 a side and 397
 // with 128 (its symmetric products 247 and 209), 2048 x 2048 x 2048 138, 49 and 81 with 64, 1536 x 1536 x 1536 symmetric 33 with 128 and 23 with 64; in
 // 8-bit integers over 4096, N tokens onto 4096 channels, quantizer included: N = 256 55, 26 and 19, 1024 60, 33 and 49, 4096 85, 115 and 174.
-// `cut`: what the last, partial round of tiles of 128 takes instead where its tiles are cut along k (CutTiles), in rounds; 0: they are not.
+// `cut`: what the last, partial round of tiles of 128 takes instead where its tiles are cut along k (CutTiles), in rounds, `few` the same of the round that
+// fewer tiles of 64 than CUs are; 0: they are not.
 inline double partial_round(double part) { return part > 0.0 ? 0.55 + 0.45 * part : 0.0; }
 template <class Tiles>
-int tile_side(const Tiles& tiles, double large, double cut = 0.0) {
+int tile_side(const Tiles& tiles, double large, double cut = 0.0, double few = 0.0) {
     const double cus = device_cu_count();
     const auto time = [&](double round, double share, double last) {
         const double whole = std::floor(share), part = share - whole;
         return round * (whole + (last > 0.0 ? last : partial_round(part)));
     };
-    const double t256 = time(large, tiles(256) / cus, 0.0), t128 = time(0.74, tiles(128) / cus, cut), t64 = 0.32 * std::fmax(1.0, tiles(64) / cus);
+    const double t256 = time(large, tiles(256) / cus, 0.0), t128 = time(0.74, tiles(128) / cus, cut), t64 = 0.32 * (few > 0.0 ? few : std::fmax(1.0, tiles(64) / cus));
     return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
 }
 
@@ -341,7 +342,7 @@ int tile_side(const Tiles& tiles, double large, double cut = 0.0) {
 struct CutTiles { int64_t whole, left; int slices, stages; double rounds; };
 inline CutTiles cut_tiles(int64_t tiles, int stages) {
     const int64_t cus = device_cu_count();
-    CutTiles c{tiles, 0, 1, stages, 0.0};
+    CutTiles c{tiles, 0, 1, stages, 0.0};                // (none is)
     const int64_t left = tiles % cus;
     if (tiles < cus || left == 0) return c;
     int64_t slices = cus / left < stages / 4 ? cus / left : stages / 4;
@@ -350,6 +351,23 @@ inline CutTiles cut_tiles(int64_t tiles, int stages) {
     slices = (stages + each - 1) / each;
     const double rounds = (each + 10.0 / 0.74) / stages;
     if (rounds < partial_round(static_cast<double>(left) / static_cast<double>(cus))) c = CutTiles{tiles - left, left, static_cast<int>(slices), each, rounds};
+    return c;
+}
+
+// ... and all tiles of 64 where they are few under a long k: a CU draws some 50 to 80 GB/s however much it has requested, so that a tile's stage of 16
+// KB takes `stage` = 0.2 (operands in the caches) to 0.32 us, and slices on other CUs draw beside it.  The join's launch and its way through memory are 3 us and
+// one for every hundred slices.  Measured, five steps without / with: 256 x 768 (10 tiles) 104 / 100 us, 256 x 2048 149 / 115, 128 x 4096 197 / 100; where the rule
+// refuses, 4 x 256 x 1024 (40) 126 / 128, 768 x 768 (78) 152 / 165.
+inline CutTiles cut_few_tiles(int64_t tiles, int stages, double stage) {
+    const int64_t cus = device_cu_count();
+    CutTiles c{tiles, 0, 1, stages, 0.0};
+    int64_t slices = tiles > 0 ? cus / tiles : 0;
+    for (const int64_t most : {static_cast<int64_t>(stages / 4), int64_t{16}}) slices = slices < most ? slices : most;
+    if (slices < 2) return c;
+    const int each = static_cast<int>((stages + slices - 1) / slices);
+    slices = (stages + each - 1) / each;
+    const double rounds = (each + (3.0 + static_cast<double>(tiles * slices) / 100.0) / stage) / stages;
+    if (rounds < 1.0) c = CutTiles{0, tiles, static_cast<int>(slices), each, rounds};
     return c;
 }
 

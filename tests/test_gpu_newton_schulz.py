@@ -84,6 +84,15 @@ def test_tiles_behind_a_whole_round(ops, shape, dtype):
     assert torch.equal(ops.newton_schulz(g, steps=2), first)
 
 
+# few tiles under a long axis are cut along it: one tile, several in a stack, a last slice that is shorter, either way round
+@pytest.mark.parametrize("shape,dtype", [((20, 1100), torch.float32), ((1, 3000), torch.float32), ((3, 70, 2010), torch.bfloat16), ((2010, 130), torch.float16), ((256, 768), torch.float32)])
+def test_long_and_thin(ops, shape, dtype):
+    g = update(shape, dtype, seed=13)
+    first = ops.newton_schulz(g, steps=3)
+    check(first, g, 3)
+    assert torch.equal(ops.newton_schulz(g, steps=3), first)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(24, 72), (3, 100, 64), (160, 160)])
 def test_types(ops, shape, dtype):
