@@ -204,12 +204,48 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const I8Rows p, int8_t
     else quantize_resident<T, R>(p, first, end, put, scale_is);
 }
 
+// Long rows: a work-group of eight waves per row, each with 256 R elements of it in registers (read twice by one wave, 30 rows of 16384 took most of 36 us)
+constexpr int I8_ROW_WAVES = 8;
+template <class T, int R>
+__global__ __launch_bounds__(I8_ROW_WAVES * 64) void i8_quantize_row_kernel(const I8Rows p, int8_t* q, int64_t q_stride, int q_end, float* scales) {
+    __shared__ float parts[I8_ROW_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k0 = 4 * static_cast<int>(threadIdx.x);
+    const T* const row = static_cast<const T*>(p.x) + static_cast<int64_t>(blockIdx.x) * p.stride;
+    typename Quad<T>::Raw raw[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) raw[i] = fetch4<T>(row, k0 + I8_ROW_WAVES * 256 * i, p.K);
+    float x[R][4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) finish4<T>(raw[i], k0 + I8_ROW_WAVES * 256 * i, p.K, x[i]);
+    RowScale scale;
+    if constexpr (sizeof(T) > 1) {
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) largest = largest_of(largest, __builtin_fabsf(x[i][e]));
+        largest = wave_butterfly(largest, [](float a, float b) { return largest_of(a, b); });
+        if (lane == 0) parts[wave] = largest;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < I8_ROW_WAVES; ++w) largest = largest_of(largest, parts[w]);
+        scale = RowScale(largest);
+        if (threadIdx.x == 0) scales[blockIdx.x] = scale.scale;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        put_row(q + static_cast<int64_t>(blockIdx.x) * q_stride, k0 + I8_ROW_WAVES * 256 * i, q_end, sizeof(T) == 1 ? pack4(x[i]) : quantize4(x[i], scale));
+}
+
 // ------------------------------------------------------------------------------------------------------------ product
 struct I8Product {
     RowBytes w, x;            // rows: channels, tokens
     const float *w_scale, *x_scale, *bias;
     void* y;                  // [tokens][channels]
     int stages, tiles_w, tiles_x;
+    // slices > 1: every tile is cut along k into work-groups of slice_stages stages, whose sums go to `sums`
+    int slices, slice_stages;
+    v4i* sums;                // [tile][slice][a wave's tiles of 16 x 16][thread]
 };
 
 // What a lane multiplies and adds to its channels of a wave's 16 TM from mw on
@@ -291,18 +327,36 @@ __device__ __forceinline__ bool whole_stores(const I8Product& p) { return p.w.ro
 template <class T, class Loop, bool DEEP>
 __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 << 10 ? Loop::WAVES / 4 : 2) void i8_product_kernel(const I8Product p) {
     constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN, PITCH = TM * 16 + 4;
+    constexpr bool CUT = DEEP && Loop::BM == 64;
     __shared__ __attribute__((aligned(128))) uint8_t even[Loop::STAGE], odd[Loop::STAGE];
     __shared__ float x_scale[Loop::BN];
-    int tm, tn;
-    tile_of(xcd_contiguous_index(blockIdx.x, p.tiles_w * p.tiles_x), p.tiles_w, p.tiles_x, tm, tn);
+    int t = xcd_contiguous_index(blockIdx.x, p.tiles_w * p.tiles_x), tm, tn, stages = p.stages;
+    RowBytes W = p.w, X = p.x;
+    if (CUT && p.slices > 1) {
+        // (slices of the same k on one XCD: they share rows of either operand)
+        t = blockIdx.x / p.slices;
+        const int first = (blockIdx.x % p.slices) * p.slice_stages;
+        W.base += first * TILE_K;
+        X.base += first * TILE_K;
+        stages = stages - first < p.slice_stages ? stages - first : p.slice_stages;
+    }
+    tile_of(t, p.tiles_w, p.tiles_x, tm, tn);
     const int m0 = tm * Loop::BM, n0 = tn * Loop::BN;
     for (int i = threadIdx.x; i < Loop::BN; i += Loop::THREADS) x_scale[i] = p.x_scale[n0 + i < p.x.rows ? n0 + i : p.x.rows - 1];
     v4i acc[TM][TN];
     if constexpr (DEEP) {
         __shared__ __attribute__((aligned(128))) uint8_t third[Loop::STAGE], fourth[Loop::STAGE];
-        Loop::run(p.w, p.x, m0, n0, p.stages, even, odd, third, fourth, acc);
+        Loop::run(W, X, m0, n0, stages, even, odd, third, fourth, acc);
+        if (CUT && p.slices > 1) {
+            v4i* const to = p.sums + static_cast<int64_t>(blockIdx.x) * (TM * TN * Loop::THREADS) + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) to[(i * TN + j) * Loop::THREADS] = acc[i][j];
+            return;
+        }
     } else {
-        Loop::run(p.w, p.x, m0, n0, p.stages, even, odd, acc);
+        Loop::run(W, X, m0, n0, stages, even, odd, acc);
     }
     const int wave = threadIdx.x >> 6, nw = wave % WN * TN * 16;
     static_assert(Loop::WAVES / 2 * 16 * PITCH * 4 <= Loop::STAGE, "half of the waves' sixteen tokens fit a stage");
@@ -311,6 +365,31 @@ __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 <<
     const Channels<T, TM> ch(p, m0 + wave / WN * TM * 16);
     if (whole_stores<T>(p)) store_tokens<true>(p, ch, lds, n0 + nw, acc, x_scale + nw);
     else                    store_tokens<false>(p, ch, lds, n0 + nw, acc, x_scale + nw);
+}
+
+// The tiles that were cut: a wave for each that one of their waves had, its slices' sums added (whole numbers: the same bits as uncut), then as above
+template <class T, class Loop>
+__global__ __launch_bounds__(64) void i8_join_kernel(const I8Product p) {
+    constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN, SUMS = TM * TN * Loop::THREADS;
+    __shared__ __attribute__((aligned(16))) float lds[16 * (TM * 16 + 4)];
+    __shared__ float x_scale[TN * 16];
+    const int lane = threadIdx.x, wave = blockIdx.x % Loop::WAVES, t = blockIdx.x / Loop::WAVES;
+    int tm, tn;
+    tile_of(t, p.tiles_w, p.tiles_x, tm, tn);
+    const int m0 = tm * Loop::BM + wave / WN * TM * 16, n0 = tn * Loop::BN + wave % WN * TN * 16;
+    if (lane < TN * 16) x_scale[lane] = p.x_scale[n0 + lane < p.x.rows ? n0 + lane : p.x.rows - 1];
+    const Channels<T, TM> ch(p, m0);
+    const v4i* const from = p.sums + static_cast<int64_t>(t) * p.slices * SUMS + wave * 64 + lane;
+    v4i acc[TM][TN] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.slices; ++s)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] += from[static_cast<int64_t>(s) * SUMS + (i * TN + j) * Loop::THREADS];
+    wave_fence();
+    if (whole_stores<T>(p)) store_tokens<true>(p, ch, lds, n0, acc, x_scale);
+    else                    store_tokens<false>(p, ch, lds, n0, acc, x_scale);
 }
 
 // Few tokens (at most 16) of long rows: what counts is the weight's way from memory.  A work-group takes 16 channels, its waves every WAVES-th stage of
@@ -522,7 +601,13 @@ template <class T>
 void launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, float* scale, int64_t waves, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), block(256);
     const int pieces = (p.K + 255) / 256;
-    if (p.K < 4 || pieces > 16) hipLaunchKernelGGL((i8_quantize_kernel<T, 0>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
+    if (pieces > 16 && pieces <= 16 * I8_ROW_WAVES && p.rows <= LAUNCH_MOST_THREADS / (64 * I8_ROW_WAVES)) {
+        const dim3 rows(static_cast<unsigned>(p.rows)), row(64 * I8_ROW_WAVES);
+        if (pieces <= 4 * I8_ROW_WAVES)      hipLaunchKernelGGL((i8_quantize_row_kernel<T, 4>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
+        else if (pieces <= 8 * I8_ROW_WAVES) hipLaunchKernelGGL((i8_quantize_row_kernel<T, 8>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
+        else                                 hipLaunchKernelGGL((i8_quantize_row_kernel<T, 16>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
+    }
+    else if (p.K < 4 || pieces > 16) hipLaunchKernelGGL((i8_quantize_kernel<T, 0>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
     else if (pieces <= 1)  hipLaunchKernelGGL((i8_quantize_kernel<T, 1>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
     else if (pieces <= 2)  hipLaunchKernelGGL((i8_quantize_kernel<T, 2>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
     else if (pieces <= 4)  hipLaunchKernelGGL((i8_quantize_kernel<T, 4>), grid, block, 0, stream, p, q, q_stride, q_end, scale);
@@ -546,8 +631,10 @@ template <class T, class Loop, bool DEEP>
 int launch_tiles(I8Product p, hipStream_t stream) {
     p.tiles_w = (p.w.rows + Loop::BM - 1) / Loop::BM;
     p.tiles_x = (p.x.rows + Loop::BN - 1) / Loop::BN;
-    if (static_cast<int64_t>(p.tiles_w) * p.tiles_x > LAUNCH_MOST_THREADS / Loop::THREADS) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
-    hipLaunchKernelGGL((i8_product_kernel<T, Loop, DEEP>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x)), dim3(Loop::THREADS), 0, stream, p);
+    if (static_cast<int64_t>(p.tiles_w) * p.tiles_x * p.slices > LAUNCH_MOST_THREADS / Loop::THREADS) { set_error("mul_mat_i8_hip: too many tiles"); return RC_BAD_ARGS; }
+    hipLaunchKernelGGL((i8_product_kernel<T, Loop, DEEP>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x * p.slices)), dim3(Loop::THREADS), 0, stream, p);
+    if constexpr (DEEP && Loop::BM == 64)
+        if (p.slices > 1) hipLaunchKernelGGL((i8_join_kernel<T, Loop>), dim3(static_cast<unsigned>(p.tiles_w * p.tiles_x * Loop::WAVES)), dim3(64), 0, stream, p);
     return check_launch("mul_mat_i8_hip");
 }
 
@@ -587,8 +674,19 @@ I8Form i8_form(int M, int N, int K) {
     return I8_TILES;
 }
 
+// Tiles of `side`; few of 64 under a long k are cut along it
+struct I8Tiles { int side; CutTiles cut; };
+I8Tiles i8_tiles(int64_t M, int64_t N, int K) {
+    const auto tiles = [&](int side) { return (M + side - 1) / side * ((N + side - 1) / side); };
+    const CutTiles few = cut_few_tiles(tiles(64), static_cast<int>(i8_row_bytes(K) / TILE_K));
+    I8Tiles t{};
+    t.side = tile_side([&](int side) { return static_cast<double>(tiles(side)); }, 2.2, 0.0, few.rounds);
+    if (t.side == 64) t.cut = few;
+    return t;
+}
+
 template <class T>
-int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* scale, I8Form form, hipStream_t stream) {
+int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* scale, I8Form form, const I8Tiles& tiles, hipStream_t stream) {
     const int row = p.stages * TILE_K;
     if (form == I8_FEW) {
         const dim3 grid(static_cast<unsigned>((p.w.rows + 15) / 16));
@@ -607,8 +705,7 @@ int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* sca
     }
     const int rc = launch_quantize(rows, q, row, row, scale, stream, "mul_mat_i8_hip");
     if (rc != RC_OK) return rc;
-    const auto tiles = [&](int side) { return static_cast<double>((p.w.rows + side - 1) / side) * static_cast<double>((p.x.rows + static_cast<int64_t>(side) - 1) / side); };
-    switch (tile_side(tiles, 2.2)) {
+    switch (tiles.side) {
         case 256: return launch_tiles<T, TilePingPong<StepI8>, false>(p, stream);
         case 128: return launch_tiles<T, TileDeep<StepI8, 2, 4, 4, 2>, true>(p, stream);
         default:  return launch_tiles<T, TileDeep<StepI8, 2, 2, 2, 2>, true>(p, stream);
@@ -644,9 +741,13 @@ extern "C" int i8_weight_pack_hip(const int8_t* w, int64_t w_stride, int M, int 
                            "i8_weight_pack_hip");
 }
 
+// (the workspace: the quantized rows, their scales, and from here on the sums of tiles that are cut)
+static int64_t i8_sums_at(int64_t N, int K) { return N * i8_row_bytes(K) + (4 * N + 15) / 16 * 16; }
+
 extern "C" size_t mul_mat_i8_workspace_hip(int M, int N, int K) {
     if (M <= 0 || M > I8_MAX_M || N <= 0 || N > I8_MAX_N || K <= 0 || K > I8_MAX_K || i8_form(M, N, K) != I8_TILES) return 0;
-    return static_cast<size_t>(N) * static_cast<size_t>(i8_row_bytes(K)) + 4 * static_cast<size_t>(N);
+    const CutTiles cut = i8_tiles(M, N, K).cut;
+    return static_cast<size_t>(i8_sums_at(N, K)) + static_cast<size_t>(cut.left * cut.slices) * (64 * 64 * 4);
 }
 
 extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const void* x, int x_type, int64_t x_stride, const float* x_scale, const float* bias,
@@ -676,9 +777,13 @@ extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const 
     p.stages = static_cast<int>(row / TILE_K);
     const I8Rows rows{x, x_type, x_stride, x_scale, N, K};
     const I8Form form = i8_form(M, N, K);
+    const I8Tiles tiles = form == I8_TILES ? i8_tiles(M, N, K) : I8Tiles{};
+    p.slices = tiles.cut.left > 0 ? tiles.cut.slices : 1;
+    p.slice_stages = tiles.cut.left > 0 ? tiles.cut.stages : p.stages;
+    p.sums = p.slices > 1 ? reinterpret_cast<v4i*>(q + i8_sums_at(N, K)) : nullptr;
     switch (y_type) {
-        case PPML_ELEM_F32:  return launch_product<float>(p, rows, q, scale, form, stream);
-        case PPML_ELEM_F16:  return launch_product<_Float16>(p, rows, q, scale, form, stream);
-        default:             return launch_product<__bf16>(p, rows, q, scale, form, stream);
+        case PPML_ELEM_F32:  return launch_product<float>(p, rows, q, scale, form, tiles, stream);
+        case PPML_ELEM_F16:  return launch_product<_Float16>(p, rows, q, scale, form, tiles, stream);
+        default:             return launch_product<__bf16>(p, rows, q, scale, form, tiles, stream);
     }
 }

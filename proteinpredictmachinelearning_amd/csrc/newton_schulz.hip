@@ -412,7 +412,7 @@ NsPlan ns_plan(int64_t batch, int64_t rows_a, int64_t rows_b, bool symmetric, in
         return symmetric ? n * (n + 1) / 2 : m * n;
     };
     const int stages = static_cast<int>(row_bytes / TILE_K);
-    const CutTiles cut = cut_tiles(batch * tiles(128), stages), few = cut_few_tiles(batch * tiles(64), stages, 0.2);
+    const CutTiles cut = cut_tiles(batch * tiles(128), stages), few = cut_few_tiles(batch * tiles(64), stages);
     NsPlan plan{};
     plan.side = tile_side([&](int side) { return static_cast<double>(batch * tiles(side)); }, 2.55, cut.rounds, few.rounds);
     plan.tiles = static_cast<int>(tiles(plan.side));

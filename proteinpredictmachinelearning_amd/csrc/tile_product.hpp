@@ -355,10 +355,11 @@ inline CutTiles cut_tiles(int64_t tiles, int stages) {
 }
 
 // ... and all tiles of 64 where they are few under a long k: a CU draws some 50 to 80 GB/s however much it has requested, so that a tile's stage of 16
-// KB takes `stage` = 0.2 (operands in the caches) to 0.32 us, and slices on other CUs draw beside it.  The join's launch and its way through memory are 3 us and
+// KB takes 0.2 us, and slices on other CUs draw beside it.  The join's launch and its way through memory are 3 us and
 // one for every hundred slices.  Measured, five steps without / with: 256 x 768 (10 tiles) 104 / 100 us, 256 x 2048 149 / 115, 128 x 4096 197 / 100; where the rule
-// refuses, 4 x 256 x 1024 (40) 126 / 128, 768 x 768 (78) 152 / 165.
-inline CutTiles cut_few_tiles(int64_t tiles, int stages, double stage) {
+// refuses, 4 x 256 x 1024 (40) 126 / 128, 768 x 768 (78) 152 / 165; in 8-bit integers 128 x 8192 -> 1024 (32) 30.6 / 25.6, 32 x 4096 -> 1024 (16) 13.5 / 12.4,
+// and 17 x 4096 -> 4096 (64), refused, 14.3 / 15.5.
+inline CutTiles cut_few_tiles(int64_t tiles, int stages) {
     const int64_t cus = device_cu_count();
     CutTiles c{tiles, 0, 1, stages, 0.0};
     int64_t slices = tiles > 0 ? cus / tiles : 0;
@@ -366,7 +367,7 @@ inline CutTiles cut_few_tiles(int64_t tiles, int stages, double stage) {
     if (slices < 2) return c;
     const int each = static_cast<int>((stages + slices - 1) / slices);
     slices = (stages + each - 1) / each;
-    const double rounds = (each + (3.0 + static_cast<double>(tiles * slices) / 100.0) / stage) / stages;
+    const double rounds = (each + (3.0 + static_cast<double>(tiles * slices) / 100.0) / 0.2) / stages;
     if (rounds < 1.0) c = CutTiles{0, tiles, static_cast<int>(slices), each, rounds};
     return c;
 }

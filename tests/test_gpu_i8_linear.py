@@ -91,6 +91,31 @@ def test_large_linear(ops, n, k, m, dtype):
     assert torch.equal(ops.mul_mat_i8(ops.I8Weight(w, ws), x[17:300], bias), got[17:300])
 
 
+# few tiles of 64 under a long k are cut along it: whole and shorter last slices, ragged sides, the longest rows
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [(30, 16384, 512), (17, 5001, 70), (40, 131071, 65), (100, 8200, 257), (17, 4096, 4096), (65, 6000, 64)])
+def test_long_rows_of_some_tokens(ops, n, k, m, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(n, k, device="cuda", generator=gen).to(dtype)
+    w, ws = weight(gen, m, k)
+    bias = torch.randn(m, device="cuda", generator=gen)
+    W = ops.I8Weight(w, ws).pack()
+    q, scale = rule(x)
+    got = ops.mul_mat_i8(W, x, bias)
+    check(got, q, scale, w, ws, bias)
+    # whole numbers add up to the same in any order: one token's bits are those of its row
+    assert torch.equal(ops.mul_mat_i8(W, x[n - 1:], bias), got[n - 1:])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.mul_mat_i8(W, x, bias)
+    for i in range(3):
+        x.copy_(x.roll(1, 0))
+        graph.replay()
+        replayed = y.clone()
+        assert torch.equal(replayed, ops.mul_mat_i8(W, x, bias)) and torch.equal(replayed, got.roll(i + 1, 0))
+
+
 @pytest.mark.parametrize("out", TYPES)
 @pytest.mark.parametrize("given", TYPES)
 def test_result_type_is_free(ops, given, out):
@@ -157,6 +182,23 @@ def test_rows_of_any_size(ops, k):
     q, s = ops.quantize_rows_i8(x.cuda())
     want_q, want_s = rule(x)
     assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [4096, 4097, 8191, 8192, 8193, 16384, 16386, 32767, 32768, 32769])
+def test_long_rows(ops, k, dtype):
+    """Every way that rows of more than a wave's registers are shared out: the largest anywhere in a row, rows that are no numbers, strided rows, a padded weight"""
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(9, k + 3, device="cuda", generator=gen).to(dtype)[:, :k]
+    for r, at in enumerate((0, k - 1, k // 2, 4095, k - 4)):
+        x[r, at] = 9.0
+    x[5, k - 1], x[6, 1], x[7] = float("nan"), float("-inf"), 0.0
+    q, s = ops.quantize_rows_i8(x)
+    want_q, want_s = rule(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(torch.nan_to_num(s.cpu(), nan=-1.0), torch.nan_to_num(want_s, nan=-1.0))
+    w = torch.randint(-128, 128, (3, k), device="cuda", generator=gen).to(torch.int8)
+    packed = ops.I8Weight(w, torch.ones(3, device="cuda")).pack()._packed
+    assert torch.equal(packed[:, :k], w) and not packed[:, k:].any()
 
 
 def test_scales_that_vanish_in_binary32(ops):
