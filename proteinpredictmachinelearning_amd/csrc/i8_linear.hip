@@ -176,7 +176,19 @@ __device__ __forceinline__ void quantize_twice(const I8Rows& p, int64_t first, i
             scale = RowScale(largest);
             scale_is(r, scale.scale);
         }
-        for (int k = 4 * lane; k < (p.K + 255) / 256 * 256; k += 256) {
+        int k = 4 * lane;
+        for (; k + 2048 <= p.K; k += 2048) {
+            typename Quad<T>::Raw raw[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) raw[u] = fetch4<T>(row, k + 256 * u, p.K);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                float x[4];
+                finish4<T>(raw[u], k + 256 * u, p.K, x);
+                put(r, k + 256 * u, sizeof(T) == 1 ? pack4(x) : quantize4(x, scale));
+            }
+        }
+        for (; k < (p.K + 255) / 256 * 256; k += 256) {
             float x[4];
             load(row, k, x);
             put(r, k, sizeof(T) == 1 ? pack4(x) : quantize4(x, scale));
@@ -204,7 +216,8 @@ __global__ __launch_bounds__(256) void i8_quantize_kernel(const I8Rows p, int8_t
     else quantize_resident<T, R>(p, first, end, put, scale_is);
 }
 
-// Long rows: a work-group of eight waves per row, each with 256 R elements of it in registers (read twice by one wave, 30 rows of 16384 took most of 36 us)
+// Long rows, and few shorter ones: a work-group of eight waves per row, each with 256 R elements of it in registers.  bf16, without / with: 30 rows of 16384
+// (read twice by one wave) 26.6 / 3.5 us, 8192 of 8192 65 / 37.5 (5.4 TB/s), 2048 of 32768 108 / 42; 64 of 4096 (one wave) 5.3 / 2.3, 1024 of 4096 6.1 / 3.8.
 constexpr int I8_ROW_WAVES = 8;
 template <class T, int R>
 __global__ __launch_bounds__(I8_ROW_WAVES * 64) void i8_quantize_row_kernel(const I8Rows p, int8_t* q, int64_t q_stride, int q_end, float* scales) {
@@ -601,9 +614,12 @@ template <class T>
 void launch_quantize(const I8Rows& p, int8_t* q, int64_t q_stride, int q_end, float* scale, int64_t waves, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((waves + 3) / 4)), block(256);
     const int pieces = (p.K + 255) / 256;
-    if (pieces > 16 && pieces <= 16 * I8_ROW_WAVES && p.rows <= LAUNCH_MOST_THREADS / (64 * I8_ROW_WAVES)) {
+    // (rows that a wave holds as well, where there are few of them)
+    if ((pieces > 16 ? p.rows <= LAUNCH_MOST_THREADS / (64 * I8_ROW_WAVES) : pieces > 4 && p.rows <= 4 * device_cu_count()) && pieces <= 16 * I8_ROW_WAVES) {
         const dim3 rows(static_cast<unsigned>(p.rows)), row(64 * I8_ROW_WAVES);
-        if (pieces <= 4 * I8_ROW_WAVES)      hipLaunchKernelGGL((i8_quantize_row_kernel<T, 4>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
+        if (pieces <= I8_ROW_WAVES)          hipLaunchKernelGGL((i8_quantize_row_kernel<T, 1>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
+        else if (pieces <= 2 * I8_ROW_WAVES) hipLaunchKernelGGL((i8_quantize_row_kernel<T, 2>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
+        else if (pieces <= 4 * I8_ROW_WAVES) hipLaunchKernelGGL((i8_quantize_row_kernel<T, 4>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
         else if (pieces <= 8 * I8_ROW_WAVES) hipLaunchKernelGGL((i8_quantize_row_kernel<T, 8>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
         else                                 hipLaunchKernelGGL((i8_quantize_row_kernel<T, 16>), rows, row, 0, stream, p, q, q_stride, q_end, scale);
     }
