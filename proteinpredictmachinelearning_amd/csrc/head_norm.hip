@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
             }
         }
     }
-    // the work-group's sums of dw, tokens in their order
+    // the work-group's sums of dw, tokens in their order, in 64 bits: a few numbers per work-group, and sums of hundreds of thousands of terms
     if (!p.partial) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -321,9 +321,9 @@ __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
         ch.template store<float>(lds + mine * p.d, dwa[s], dwb[s]);
         __syncthreads();
         for (int e = threadIdx.x; e < p.d; e += 256) {
-            float sum = 0.0f;
-            for (int g = 0; g < groups; ++g) sum += lds[g * p.d + e];
-            p.partial[(static_cast<int64_t>(blockIdx.y * gridDim.x + blockIdx.x) * 2 + s) * p.d + e] = sum;
+            double sum = 0.0;
+            for (int g = 0; g < groups; ++g) sum += static_cast<double>(lds[g * p.d + e]);
+            p.partial[(static_cast<int64_t>(blockIdx.y * gridDim.x + blockIdx.x) * 2 + s) * p.d + e] = static_cast<float>(sum);
         }
     }
 }
@@ -331,26 +331,26 @@ __global__ __launch_bounds__(256) void head_norm_back_kernel(const HeadNorm p) {
 // dw[e] = the sum over `parts` work-groups of partial[part][side][e].  A work-group takes eight elements, 32 threads each: a thread every 32nd part,
 // eight of them on their way at once (a chain of loads 21 us for 1024 parts of 32 elements).
 __global__ __launch_bounds__(256) void head_norm_weights_kernel(const float* partial, int parts, int d, float* dwq, float* dwk) {
-    __shared__ float lds[32][9];
+    __shared__ double lds[32][9];
     const int col = threadIdx.x & 7, run = threadIdx.x >> 3;
     const int e = blockIdx.x * 8 + col, s = blockIdx.y;
     float* const dw = s == 0 ? dwq : dwk;
     if (!dw) return;
     const float* const from = partial + s * d + (e < d ? e : d - 1);
     const int64_t step = 2 * static_cast<int64_t>(d);
-    float sum = 0.0f;
+    double sum = 0.0;
     for (int i = run; i < parts; i += 32 * 8) {
         float x[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) x[u] = from[(i + 32 * u < parts ? i + 32 * u : run) * step];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) sum += i + 32 * u < parts ? x[u] : 0.0f;
+        for (int u = 0; u < 8; ++u) sum += i + 32 * u < parts ? static_cast<double>(x[u]) : 0.0;
     }
     lds[run][col] = sum;
     __syncthreads();
     if (run == 0 && e < d) {
         for (int i = 1; i < 32; ++i) sum += lds[i][col];
-        dw[e] = sum;
+        dw[e] = static_cast<float>(sum);
     }
 }
 

@@ -307,7 +307,7 @@ __device__ __forceinline__ void ns_finish_block(const NsProduct& p, float* lds, 
 
 // One of a step's three products.  Large matrices are bound by the matrix pipe and its power.  Traced at 4096 x 4096: B X in tiles of 256 a side 321 us (1.29
 // PFLOP/s of f16 products; the library's large f16 product 1.37), A and A A in tiles of 128 on and above the diagonal 187 us and 8 of the join (1.14 without it).  Small
-// matrices are a chain of 17 launches of 6 to 8 us each (768 x 256): 2.3 of a launch, a way to memory, 4 to 24 stages, and the way out.
+// matrices are a chain of 17 launches (22 with joins) of 4 to 6 us each (768 x 256): 2.3 of a launch, a way to memory, 4 to 8 stages, and the way out.
 template <class T, class Loop, bool DEEP>
 __global__ __launch_bounds__(Loop::THREADS, Loop::STAGE * (DEEP ? 4 : 2) > 80 << 10 ? Loop::WAVES / 4 : 2) void ns_product_kernel(const NsProduct p) {
     constexpr int WN = Loop::WN, TM = Loop::TM, TN = Loop::TN;
