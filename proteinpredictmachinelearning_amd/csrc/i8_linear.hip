@@ -518,7 +518,7 @@ __global__ __launch_bounds__(I8_FEW_WAVES * 64) void i8_few_kernel(const I8Produ
 // into LDS by all its waves, and every wave multiplies them with its channels.  One launch, x read once (once per part of 64 WAVES channels).
 // A wave quantizes four rows at a time, sixteen lanes each: the search for the largest then takes four steps for four rows (a row
 // at a time by 64 lanes, six steps each, the alignment's projection was bound by it: 39 us).  Traced: 26368 tokens of 256, f32, onto 768 channels 24.3 us
-// (4.4 TB/s); 408 onto 256 4.4 us; 2601 of 500, f16, onto 1001 11.9 us (rows that no piece of sixteen bytes divides).
+// (4.4 TB/s); 408 onto 256 4.4 us.
 template <class T, bool VEC, int S, int WAVES, int TM>
 __global__ __launch_bounds__(WAVES * 64) void i8_stay_kernel(const I8Product p, const I8Rows rows) {
     constexpr int TN = WAVES / 4, TOKENS = TN * 16, PITCH = TM * 16 + 4, ROW = S * TILE_K, LDS_ROW = ROW + 16;
@@ -685,6 +685,10 @@ constexpr int I8_FEW_LDS = 40 << 10, I8_STAY_STAGES = 4;
 I8Form i8_form(int M, int N, int K) {
     const int64_t row = i8_row_bytes(K);
     if (K < 4) return I8_TILES;                         // (the rows are fetched four elements at a time)
+    // (tiles behind a quantizing launch / staying, f16, us: 2601 tokens of 512 onto 512 channels 9.2 / 10.2, onto 1024 10.7 / 12.8, onto 4096 21.3 / 24.2; on either side of
+    // the range 512 onto 1024 7.6 / 5.5, 10000 onto 1024 23.7 / 23.4, 30000 onto 512 29.9 / 27.4)
+    const int64_t outputs = static_cast<int64_t>(N) * M;
+    if (row > 2 * TILE_K && row <= I8_STAY_STAGES * TILE_K && M > 256 && outputs >= 1 << 20 && outputs <= 11 << 20) return I8_TILES;
     if (row <= I8_STAY_STAGES * TILE_K && (M + 511) * row < 0x7fffffff) return I8_STAY;
     if (N <= 16 && row <= I8_FEW_PART * few_share(N) && N * (row + 16) <= I8_FEW_LDS) return I8_FEW;
     return I8_TILES;
@@ -702,7 +706,7 @@ I8Tiles i8_tiles(int64_t M, int64_t N, int K) {
 }
 
 template <class T>
-int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* scale, I8Form form, const I8Tiles& tiles, hipStream_t stream) {
+int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* scale, I8Form form, const I8Tiles& tiles, bool in_place, hipStream_t stream) {
     const int row = p.stages * TILE_K;
     if (form == I8_FEW) {
         const dim3 grid(static_cast<unsigned>((p.w.rows + 15) / 16));
@@ -719,8 +723,10 @@ int launch_product(const I8Product& p, const I8Rows& rows, int8_t* q, float* sca
         else                    launch_stay<T, 4>(p, rows, stream);
         return check_launch("mul_mat_i8_hip");
     }
-    const int rc = launch_quantize(rows, q, row, row, scale, stream, "mul_mat_i8_hip");
-    if (rc != RC_OK) return rc;
+    if (!in_place) {
+        const int rc = launch_quantize(rows, q, row, row, scale, stream, "mul_mat_i8_hip");
+        if (rc != RC_OK) return rc;
+    }
     switch (tiles.side) {
         case 256: return launch_tiles<T, TilePingPong<StepI8>, false>(p, stream);
         case 128: return launch_tiles<T, TileDeep<StepI8, 2, 4, 4, 2>, true>(p, stream);
@@ -792,14 +798,22 @@ extern "C" int mul_mat_i8_hip(const int8_t* packed, const float* w_scale, const 
     p.y = y;
     p.stages = static_cast<int>(row / TILE_K);
     const I8Rows rows{x, x_type, x_stride, x_scale, N, K};
-    const I8Form form = i8_form(M, N, K);
+    I8Form form = i8_form(M, N, K);
+    // Quantized rows that lie as tiles read them are read where they are: tiles then need no launch before them, and no workspace where they are not cut
+    const bool in_place = x_type == PPML_ELEM_I8 && K % TILE_K == 0 && x_stride % 16 == 0 && x_stride <= 1 << 20 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    if (in_place) {
+        p.x = RowBytes{static_cast<const uint8_t*>(x), x_stride, N};
+        // (tiles / staying, us: 2601 x 512 -> 1024 6.4 / 10.5, 30000 x 512 -> 512 16.7 / 24.5, 100 x 512 -> 1024 3.6 / 5.1, 30000 x 512 -> 128 8.0 / 15.7, 26368 x 256 -> 256
+        // 11.2 / 12.0, -> 768 23.8 / 22.8, 5000 x 256 -> 2048 13.7 / 13.6, 10609 x 128 -> 512 9.6 / 8.4)
+        if (form == I8_STAY && N >= 64 && (row > 2 * TILE_K || (row == 2 * TILE_K && static_cast<int64_t>(N) * M <= 8 << 20))) form = I8_TILES;
+    }
     const I8Tiles tiles = form == I8_TILES ? i8_tiles(M, N, K) : I8Tiles{};
     p.slices = tiles.cut.left > 0 ? tiles.cut.slices : 1;
     p.slice_stages = tiles.cut.left > 0 ? tiles.cut.stages : p.stages;
     p.sums = p.slices > 1 ? reinterpret_cast<v4i*>(q + i8_sums_at(N, K)) : nullptr;
     switch (y_type) {
-        case PPML_ELEM_F32:  return launch_product<float>(p, rows, q, scale, form, tiles, stream);
-        case PPML_ELEM_F16:  return launch_product<_Float16>(p, rows, q, scale, form, tiles, stream);
-        default:             return launch_product<__bf16>(p, rows, q, scale, form, tiles, stream);
+        case PPML_ELEM_F32:  return launch_product<float>(p, rows, q, scale, form, tiles, in_place, stream);
+        case PPML_ELEM_F16:  return launch_product<_Float16>(p, rows, q, scale, form, tiles, in_place, stream);
+        default:             return launch_product<__bf16>(p, rows, q, scale, form, tiles, in_place, stream);
     }
 }

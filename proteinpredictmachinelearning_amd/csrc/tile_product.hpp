@@ -7,10 +7,10 @@
 
 namespace ppmlhip {
 
-// A dense operand: rows of bytes along k, zero from the last k on to a whole number of 128.
+// An operand: rows of a whole number of 128 bytes along k, zero from the last k on.
 struct RowBytes {
     const uint8_t* base;
-    int64_t stride;           // bytes from row to row: a multiple of 128
+    int64_t stride;           // bytes from row to row: a multiple of 16
     int rows;
 };
 

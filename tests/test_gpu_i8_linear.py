@@ -184,6 +184,23 @@ def test_rows_of_any_size(ops, k):
     assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
 
 
+@pytest.mark.parametrize("n,k,m", [(600, 512, 1030), (513, 384, 1029), (2600, 512, 500), (4100, 128, 4100), (4100, 640, 4200), (40, 8192, 257), (300, 1152, 300), (1, 512, 700), (2, 100, 3000)])
+def test_quantized_rows_where_they_lie(ops, n, k, m):
+    """Dense, strided and shifted rows of quantized activations, whether or not they can be read in place: the bits of quantizing on the way; what is behind and between rows plays no part"""
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    x = torch.randn(n, k, device="cuda", generator=gen)
+    W = ops.I8Weight(*weight(gen, m, k)).pack()
+    bias = torch.randn(m, device="cuda", generator=gen)
+    want = ops.mul_mat_i8(W, x, bias)
+    q, s = ops.quantize_rows_i8(x)
+    assert torch.equal(ops.mul_mat_i8(W, (q, s), bias), want)
+    for extra, at in ((16, 0), (16, 16), (128, 64), (8, 0), (16, 8), (3, 1)):
+        wide = torch.randint(-128, 128, (n, k + extra), device="cuda", generator=gen).to(torch.int8)
+        part = wide[:, min(at, extra):][:, :k]
+        part.copy_(q)
+        assert torch.equal(ops.mul_mat_i8(W, (part, s), bias), want), (extra, at)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("k", [4096, 4097, 8191, 8192, 8193, 16384, 16386, 32767, 32768, 32769])
 def test_long_rows(ops, k, dtype):
